@@ -63,6 +63,10 @@ extern "C" {
 #define CTN_EPI_NORMBWD 5    /* Y = acc; norm-backward sums of g = egamma*acc and g*xhat(E): esums / ecol */
 #define CTN_EPI_ADD 6        /* Y = acc + bias + (R ? R : 0) */
 
+/* element types of the frame norm, rotary and attention entry points */
+#define CTN_TYPE_F32 0
+#define CTN_TYPE_BF16 1
+
 const char* ctn_version(void);
 const char* ctn_last_error(void);
 /* sizeof() of the argument structs below, for bindings to check their mirror of this header */
@@ -229,6 +233,70 @@ int ctn_rows_gemm(const float* X, int64_t ldx, const float* W, int64_t ldw, int 
                   int K, int M, float* Y, int64_t ldy, int arith, void* stream);
 int ctn_rows_wgrad(const float* dY, int64_t lddy, const float* X, int64_t ldx, int64_t R, int M, int K, float* dW,
                    int64_t lddw, float* dbias, float sign, int arith, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Operators of the attention form of the dual-path unit.  The reference has no counterpart: its dual-path blocks walk their
+ * axes with an nn.LSTM (src/models/dprnn.py:60-64, :104-114); these take its place between the unit's axis shuffles
+ * and its linear layer.  `type` is CTN_TYPE_F32 or CTN_TYPE_BF16 (all tensors of a call), strides are in elements, sums and
+ * statistics fp32.
+ *
+ * ctn_frame_norm_*: layer norm over the C features of each of R rows (row strides ldx, ldy, lddy, lddx >= C; any
+ * alignment; 1 <= C <= 16384):  y = (x - mean) / sqrt(var + eps) * gamma + beta.  gamma / beta may be null (ones / zeros);
+ * wtype, CTN_TYPE_F32 or `type`, is their type and that of their gradients.  stats: 3 R floats for the backward pass (mean, the mean's
+ * own rounding error, 1 / sqrt(var + eps)); may be null in the forward call.  The backward call writes dx, dgamma and dbeta
+ * (each may be null); for dgamma / dbeta it wants a workspace of ctn_frame_norm_bwd_ws_floats(R, C, type) floats, contents
+ * irrelevant before and after, one per call that may run concurrently; they are summed in a fixed order.
+ * ------------------------------------------------------------------------------------------- */
+int ctn_frame_norm_fwd(const void* x, int64_t ldx, int64_t R, int C, int type, const void* gamma, const void* beta, int wtype,
+                       float eps, void* y, int64_t ldy, float* stats, void* stream);
+int64_t ctn_frame_norm_bwd_ws_floats(int64_t R, int C, int type);
+int ctn_frame_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, int type,
+                       const void* gamma, int wtype, const float* stats, void* dx, int64_t lddx, void* dgamma, void* dbeta,
+                       float* ws, int64_t ws_floats, void* stream);
+
+/* ctn_rotary: y = x with the pairs of every head's first `rotary` elements (even, <= D) turned by 2 pi p turns[i] and scaled
+ * by `magnitude`; the other elements are copied.  x, y (B, T, H, D) by strides with unit feature stride, any alignment;
+ * y == x with equal strides is allowed.  Token t of batch element b is at position p = positions[b * pbs + t]
+ * (pbs = 0: one row of positions for all), or first + t when positions is null.  turns: rotary / 2 doubles, turns per
+ * position.  interleaved = 0: pair i is elements (i, i + rotary / 2), 1: (2 i, 2 i + 1).  inverse = 1 turns the other way:
+ * the gradient of the map.  Positions up to 2^31 in magnitude keep fp32 accuracy. */
+int ctn_rotary(const void* x, int64_t xbs, int64_t xts, int64_t xhs, int B, int T, int H, int D, int type,
+               const int64_t* positions, int64_t pbs, int64_t first, const double* turns, int rotary, int interleaved,
+               int inverse, float magnitude, void* y, int64_t ybs, int64_t yts, int64_t yhs, void* stream);
+
+/* ctn_attn_*: o[b][i][h] = sum_j p_ij v[b][j][h / (H / Hk)], p = softmax over the visible keys of scale q_i . k_j.  Key j is
+ * visible to query i when j < lengths[b] (int32, clamped to 0 .. Tk; null: Tk) and, if causal, j <= i + Tk - Tq (the last
+ * query sees the last key).  A row that sees no key is zero and has zero gradients.  Keys and values at or behind
+ * lengths[b] are never read; a causal mask hides scores only: a NaN or infinity in v (or k, in the backward pass) behind a query's last key but
+ * before lengths[b] may reach it.
+ * q, o, d_o, dq (batch, Tq, H, D), k, v, dk, dv (batch, Tk, Hk, D) by strides (batch, token, head) with unit feature stride,
+ * 16-byte aligned, strides multiples of 16 bytes; D a multiple of 8 up to 128, H a multiple of Hk, scale > 0.
+ * lse (batch, H, Tq) floats: log2 of the row's sum of exp(score), -infinity for a row that sees nothing; may be null in the
+ * forward call, read by the backward call, which recomputes the probabilities from it.
+ * ws: workspace of ctn_attn_fwd_ws_floats / ctn_attn_bwd_ws_floats floats (16-byte aligned, contents irrelevant before and
+ * after, one per call that may run concurrently); -1 from these means arguments that the call would refuse.
+ * Results do not depend on the order of blocks: the same bits on every run. */
+typedef struct {
+    int32_t batch, Tq, Tk, H, Hk, D, type, causal;
+    float scale;
+    int32_t pad0;
+    const int32_t* lengths;
+    const void* q; int64_t q_b, q_t, q_h;
+    const void* k; int64_t k_b, k_t, k_h;
+    const void* v; int64_t v_b, v_t, v_h;
+    void* o; int64_t o_b, o_t, o_h;
+    float* lse;
+    const void* d_o; int64_t do_b, do_t, do_h;
+    void* dq; int64_t dq_b, dq_t, dq_h;
+    void* dk; int64_t dk_b, dk_t, dk_h;
+    void* dv; int64_t dv_b, dv_t, dv_h;
+    float* ws; int64_t ws_floats;
+} ctn_attn_args;
+int ctn_sizeof_attn_args(void);
+int64_t ctn_attn_fwd_ws_floats(const ctn_attn_args* args);
+int ctn_attn_fwd(const ctn_attn_args* args, void* stream);
+int64_t ctn_attn_bwd_ws_floats(const ctn_attn_args* args);
+int ctn_attn_bwd(const ctn_attn_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Backward pass of a residual layer's two pointwise heads in one launch: what ctn_gemm_nn (heads' input gradient with the

@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("CTN_LIB", os.path.join(_HERE, "libctn_hip.so"))   # C
 
 XF_PRELU, XF_NORM, XF_NORMBWD = 1, 2, 4
 ARITH_DEFAULT, ARITH_F32, ARITH_BF16X2, ARITH_BF16X3 = 0, 1, 2, 3     # CTN_ARITH_* of include/ctn.h
+TYPE_F32, TYPE_BF16 = 0, 1                                            # CTN_TYPE_* of include/ctn.h
 STAT_SLOTS = 32          # CTN_STAT_SLOTS of include/ctn.h
 PIT_NOALLOC_MAX_WORK = 65536   # CTN_PIT_NOALLOC_MAX_WORK of include/ctn.h
 EPI_STORE, EPI_STATS, EPI_HEADS, EPI_SIGMOID, EPI_PRELUBWD, EPI_NORMBWD, EPI_ADD = range(7)
@@ -155,6 +156,24 @@ class HeadsBwdArgs(C.Structure):
     ]
 
 
+class AttnArgs(C.Structure):
+    _fields_ = [
+        ("batch", _i32), ("Tq", _i32), ("Tk", _i32), ("H", _i32), ("Hk", _i32), ("D", _i32), ("type", _i32), ("causal", _i32),
+        ("scale", _f32), ("pad0", _i32),
+        ("lengths", _p),
+        ("q", _p), ("q_b", _i64), ("q_t", _i64), ("q_h", _i64),
+        ("k", _p), ("k_b", _i64), ("k_t", _i64), ("k_h", _i64),
+        ("v", _p), ("v_b", _i64), ("v_t", _i64), ("v_h", _i64),
+        ("o", _p), ("o_b", _i64), ("o_t", _i64), ("o_h", _i64),
+        ("lse", _p),
+        ("d_o", _p), ("do_b", _i64), ("do_t", _i64), ("do_h", _i64),
+        ("dq", _p), ("dq_b", _i64), ("dq_t", _i64), ("dq_h", _i64),
+        ("dk", _p), ("dk_b", _i64), ("dk_t", _i64), ("dk_h", _i64),
+        ("dv", _p), ("dv_b", _i64), ("dv_t", _i64), ("dv_h", _i64),
+        ("ws", _p), ("ws_floats", _i64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/ctn.h declares
 PROTOTYPES = {
     "ctn_version": (C.c_char_p, []),
@@ -221,6 +240,17 @@ PROTOTYPES = {
                                          C.c_int, _p, _i64, _i64, C.c_int, _p, _i64, _i64, _p, _p, _p]),
     "ctn_pair_sdr_fwd": (C.c_int, [_p, _p, C.c_int, C.c_int, C.c_int, _i64, _i64, _f32, C.c_int, _p, _p, _p, _p]),
     "ctn_pair_sdr_bwd": (C.c_int, [_p, _p, C.c_int, C.c_int, C.c_int, _i64, _i64, _p, _p, _p, _i64, _i64, _p]),
+    "ctn_frame_norm_fwd": (C.c_int, [_p, _i64, _i64, C.c_int, C.c_int, _p, _p, C.c_int, _f32, _p, _i64, _p, _p]),
+    "ctn_frame_norm_bwd_ws_floats": (_i64, [_i64, C.c_int, C.c_int]),
+    "ctn_frame_norm_bwd": (C.c_int, [_p, _i64, _p, _i64, _i64, C.c_int, C.c_int, _p, C.c_int, _p, _p, _i64, _p, _p, _p, _i64,
+                                     _p]),
+    "ctn_rotary": (C.c_int, [_p, _i64, _i64, _i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _p, _i64, _i64, _p, C.c_int,
+                             C.c_int, C.c_int, _f32, _p, _i64, _i64, _i64, _p]),
+    "ctn_sizeof_attn_args": (C.c_int, []),
+    "ctn_attn_fwd_ws_floats": (_i64, [C.POINTER(AttnArgs)]),
+    "ctn_attn_fwd": (C.c_int, [C.POINTER(AttnArgs), _p]),
+    "ctn_attn_bwd_ws_floats": (_i64, [C.POINTER(AttnArgs)]),
+    "ctn_attn_bwd": (C.c_int, [C.POINTER(AttnArgs), _p]),
     "ctn_sumsq": (C.c_int, [_p, _i64, _p, _p]),
     "ctn_adam_step": (C.c_int, [_p, _p, _p, _p, _i64, _p, _f32, _f32, _f32, _f32, _f32, _f32, C.c_int, _p]),
 }
@@ -233,6 +263,7 @@ _STRUCT_SIZES = {
     "ctn_sizeof_heads_bwd_args": HeadsBwdArgs,
     "ctn_sizeof_wprep_item": WPrepItem,
     "ctn_sizeof_transpose_item": TransposeItem,
+    "ctn_sizeof_attn_args": AttnArgs,
 }
 
 _lib = None

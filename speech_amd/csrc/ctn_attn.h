@@ -1,0 +1,191 @@
+// Pieces shared by the attention kernels (ctn_attn_fwd.hip, ctn_attn_bwd.hip), gfx950.
+//
+// All products run on v_mfma_f32_32x32x16_bf16 with fp32 accumulation.  bf16 tensors feed it as they are; fp32 tensors as
+// three exact bf16 pieces, x = hi + mid + lo (each the next eight significant bits), and the six products of pieces above
+// 2^-22 of the largest -- the arithmetic CTN_ARITH_BF16X3 of the framework's GEMMs.
+//
+// Fragment layouts of the instruction: A[m = lane % 32][k = 8 (lane / 32) + j], B[k = 8 (lane / 32) + j][n = lane % 32],
+// j = 0 .. 7; accumulator element e of a lane is row (e & 3) + 8 (e >> 2) + 4 (lane / 32) of column lane % 32.
+// The kernels compute scores with the axis they keep (queries in the forward pass and dQ, keys in dK / dV) as COLUMNS:
+// a lane then owns one row of the softmax, its statistics need one exchange between the half-waves, and its eight
+// accumulator values 8 s .. 8 s + 7 are the B fragment of contraction step s of the next product once the other operand
+// uses the same order of contraction indices: slot (half, j) is index 16 s + 4 half + (j & 3) + 8 (j >> 2).
+#pragma once
+#include "ctn_common.h"
+
+namespace attn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> struct Planes;
+template <> struct Planes<float> { static constexpr int N = 3; };
+template <> struct Planes<__bf16> { static constexpr int N = 1; };
+
+template <int NP> struct Frag { bf16x8 p[NP]; };
+
+__device__ __forceinline__ void mma(f32x16& acc, const Frag<1>& a, const Frag<1>& b) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& acc, const Frag<3>& a, const Frag<3>& b) {      // smallest products first
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
+}
+
+// eight fp32 values as a fragment: rounded to nearest bf16 (at most half a step, 2^-8 of a value), or split exactly
+__device__ __forceinline__ void make_frag(const float (&x)[8], Frag<1>& f) {
+    union { bf16x8 v; bf16x2 h[4]; } u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u.h[i] = __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2);
+    f.p[0] = u.v;
+}
+__device__ __forceinline__ void make_frag(const float (&x)[8], Frag<3>& f) {
+    union { bf16x8 v; unsigned u[4]; } h, m, l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned x0 = __float_as_uint(x[2 * i]), x1 = __float_as_uint(x[2 * i + 1]);
+        h.u[i] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+        const float r0 = x[2 * i] - __uint_as_float(x0 & 0xffff0000u), r1 = x[2 * i + 1] - __uint_as_float(x1 & 0xffff0000u);
+        const unsigned y0 = __float_as_uint(r0), y1 = __float_as_uint(r1);
+        m.u[i] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+        const float q0 = r0 - __uint_as_float(y0 & 0xffff0000u), q1 = r1 - __uint_as_float(y1 & 0xffff0000u);
+        l.u[i] = __builtin_amdgcn_perm(__float_as_uint(q1), __float_as_uint(q0), 0x07060302u);
+    }
+    f.p[0] = h.v, f.p[1] = m.v, f.p[2] = l.v;
+}
+
+// eight consecutive elements as they lie in memory
+template <typename T> struct Chunk;
+template <> struct Chunk<__bf16> {
+    u32x4 v;
+    __device__ __forceinline__ void load(const __bf16* p) { v = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void zero() { v = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void frag(Frag<1>& f) const { f.p[0] = __builtin_bit_cast(bf16x8, v); }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        const bf16x8 b = __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)b[i];
+    }
+};
+template <> struct Chunk<float> {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = ctn_ld4(p), b = ctn_ld4(p + 4); }
+    __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    }
+    __device__ __forceinline__ void frag(Frag<3>& f) const {
+        float x[8];
+        floats(x);
+        make_frag(x, f);
+    }
+};
+
+// LDS image of a plane of rows of DT bf16: the 16-byte chunk ch of row r lies at chunk ch ^ key(r) of its row.  The keys
+// put the chunks of one column of 16 consecutive rows (a plain fragment read) and the 4 rows x 4 chunks of a transposing
+// read on distinct banks.
+template <int DT> __device__ __forceinline__ int img(const int r, const int ch) {
+    static_assert(DT == 32 || DT == 64 || DT == 128, "head tile");
+    const int key = DT == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : DT == 64 ? ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : ((r >> 2) & 3);
+    return 2 * DT * r + 16 * (ch ^ key);
+}
+
+// Tile of ROWS x DT elements staged by NT threads: thread's chunk i is chunk (tid + NT i) of the tile, row by row
+template <typename T, int DT, int ROWS, int NT> struct Tile {
+    static constexpr int CPR = DT / 8, N = ROWS * CPR / NT, PLANE = ROWS * DT * 2;
+    static constexpr int BYTES = Planes<T>::N * PLANE;
+    static_assert(ROWS * CPR % NT == 0, "whole chunks per thread");
+    Chunk<T> c[N];
+    // rows 0 .. nvalid - 1 at base + row * stride, D elements each; everything else zero
+    __device__ __forceinline__ void load(const T* __restrict__ base, const int64_t stride, const int nvalid, const int D) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int q = threadIdx.x + NT * i, r = q / CPR, d = (q % CPR) * 8;
+            if (r < nvalid && d < D) c[i].load(base + r * stride + d);
+            else c[i].zero();
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int q = threadIdx.x + NT * i, r = q / CPR, ch = q % CPR;
+            Frag<Planes<T>::N> f;
+            c[i].frag(f);
+#pragma unroll
+            for (int p = 0; p < Planes<T>::N; ++p) *reinterpret_cast<bf16x8*>(lds + p * PLANE + img<DT>(r, ch)) = f.p[p];
+        }
+    }
+};
+
+// A fragment of rows r0 .. r0 + 31, contraction step s along the row
+template <int NP, int DT, int ROWS>
+__device__ __forceinline__ void frag_rows(const unsigned char* lds, const int r0, const int s, Frag<NP>& f) {
+    const int lane = threadIdx.x & 63;
+    const int o = img<DT>(r0 + (lane & 31), 2 * s + (lane >> 5));
+#pragma unroll
+    for (int p = 0; p < NP; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(lds + p * (ROWS * DT * 2) + o);
+}
+// A fragment of columns c0 .. c0 + 31 (transposed view), contraction over rows r0 .. r0 + 15 in the accumulators' order:
+// ds_read_b64_tr_b16, per group of 16 lanes a block of 4 rows x 16 columns that comes back column by column (lane 4 q + p
+// of the group supplies the address of row q, columns 4 p .. 4 p + 3)
+template <int NP, int DT, int ROWS>
+__device__ __forceinline__ void frag_cols(const unsigned char* lds, const int r0, const int c0, Frag<NP>& f) {
+    const int lane = threadIdx.x & 63;
+    const int col = c0 + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        union { bf16x8 v; s16x4 h[2]; } u;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int row = r0 + 8 * x + 4 * (lane >> 5) + ((lane & 15) >> 2);
+            const unsigned char* ptr = lds + p * (ROWS * DT * 2) + img<DT>(row, col >> 3) + (col & 4) * 2;
+            u.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(ptr));
+        }
+        f.p[p] = u.v;
+    }
+}
+
+// row of accumulator element e
+__device__ __forceinline__ int acc_row(const int e) { return (e & 3) + 8 * (e >> 2) + 4 * ((threadIdx.x & 63) >> 5); }
+
+// value of this lane's column in the other half-wave
+__device__ __forceinline__ float half_max(const float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(const float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// four consecutive elements of an output row (16- or 8-byte aligned)
+__device__ __forceinline__ void store4(float* p, const f32x4 v) { ctn_st4(p, v); }
+__device__ __forceinline__ void store4(__bf16* p, const f32x4 v) {
+    union { unsigned long long u; bf16x2 h[2]; } x;
+    x.h[0] = __builtin_convertvector(f32x2{v[0], v[1]}, bf16x2), x.h[1] = __builtin_convertvector(f32x2{v[2], v[3]}, bf16x2);
+    *reinterpret_cast<unsigned long long*>(p) = x.u;
+}
+
+// Block index -> work index: blocks are dealt to the eight dies in turn, each die gets a contiguous stretch of the work,
+// so that the blocks that share keys share a die's L2.
+__device__ __forceinline__ unsigned die_order(const unsigned id, const unsigned n) {
+    const unsigned q = n >> 3, r = n & 7, x = id & 7, i = id >> 3;
+    return x < r ? x * (q + 1) + i : r * (q + 1) + (x - r) * q + i;
+}
+
+static inline bool strides_ok(const void* p, int64_t b, int64_t t, int64_t h, int es) {
+    const int64_t m = 16 / es;
+    return ctn_aligned16(p) && b % m == 0 && t % m == 0 && h % m == 0 && b >= 0 && t >= 0 && h >= 0;
+}
+
+}  // namespace attn

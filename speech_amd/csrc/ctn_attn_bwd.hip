@@ -1,0 +1,377 @@
+// Attention, backward, gfx950.  From the forward pass's log-sums the probabilities are formed again, tile by tile:
+//
+//   p_ij = exp(scale q_i . k_j - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i
+//
+// Two launches, each with the axis it keeps as the columns of its scores (ctn_attn.h), so that neither probabilities nor
+// score gradients leave the registers and every sum has one owner and a fixed order: the dQ kernel walks key tiles (and
+// forms delta on the way, for the second launch), the dK / dV kernel walks the query tiles of all query heads of its key
+// head.  Seven products where an order-free accumulation of dQ would need five: the price of the same bits on every run.
+// For bf16 tensors p and ds are rounded to bf16 (half a step, relative 2^-8 each at most) where they enter a product.
+#include "ctn_attn.h"
+
+bool ctn_attn_args_ok(const ctn_attn_args* a, const char* who);
+
+namespace {
+using namespace attn;
+
+// rows of the walked tiles: 64, or 32 where two buffers of 64 would take more than half of the LDS
+template <typename T, int DT> constexpr int walk_tile() { return Planes<T>::N * DT <= 128 ? 64 : 32; }
+
+struct bwd_params {
+    ctn_attn_args a;
+    int G, nt;               // tiles of the kept axis per (batch element, head)
+    float sl2;
+    float* delta;            // [B][H][Tq]
+};
+
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const bwd_params f) {
+    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, KT = walk_tile<T, DT>();
+    typedef Tile<T, DT, KT, NT> tile_t;
+    constexpr int BUF = 2 * tile_t::BYTES;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
+    const ctn_attn_args& a = f.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int off = a.Tk - a.Tq;
+    unsigned id = die_order(blockIdx.x, gridDim.x);
+    const int qt = f.nt - 1 - (int)(id % f.nt);
+    id /= f.nt;
+    const int head = id % a.H, b = id / a.H, hk = head / f.G;
+    const int w0 = qt * 32 * NW + wave * 32, tq = w0 + (lane & 31);
+    const bool live = tq < a.Tq;
+
+    int len = a.Tk;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
+    const int vis = !live ? 0 : a.causal ? min(len, tq + off + 1) : len;
+    int kend = len, wfull = len, wend = len;
+    if (a.causal) {
+        kend = min(len, min(a.Tq, (qt + 1) * 32 * NW) + off);
+        wfull = min(len, w0 + off + 1);
+        wend = min(len, min(a.Tq, w0 + 32) + off);
+    }
+    if (w0 >= a.Tq) wend = 0;
+    const int t1 = kend > 0 ? (kend + KT - 1) / KT : 0;
+
+    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h;
+    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h;
+    tile_t tk, tv;
+    auto fetch = [&](const int t) {
+        tk.load(kp + (int64_t)t * KT * a.k_t, a.k_t, kend - t * KT, a.D);
+        tv.load(vp + (int64_t)t * KT * a.v_t, a.v_t, kend - t * KT, a.D);
+    };
+    auto stage = [&](const int buf) {
+        tk.store(lds + buf * BUF);
+        tv.store(lds + buf * BUF + tile_t::BYTES);
+    };
+    if (t1 > 0) fetch(0);
+
+    Frag<NP> q[KS], g[KS];
+    float delta = 0.f;
+    {
+        const T* qp = (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
+        const T* gp = (const T*)a.d_o + b * a.do_b + tq * a.do_t + head * a.do_h;
+        const T* op = (const T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * half;
+            Chunk<T> cq, cg, co;
+            if (live && d < a.D) cq.load(qp + d), cg.load(gp + d), co.load(op + d);
+            else cq.zero(), cg.zero(), co.zero();
+            cq.frag(q[s]);
+            cg.frag(g[s]);
+            float x[8], y[8];
+            cg.floats(x);
+            co.floats(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
+        }
+    }
+    delta = half_sum(delta);
+    const int64_t row = ((int64_t)b * a.H + head) * a.Tq + tq;
+    float lse = live ? a.lse[row] : INFINITY;
+    if (lse == -INFINITY) lse = INFINITY;            // a row that sees nothing: every probability comes out as zero
+    if (live && half == 0) f.delta[row] = delta;
+
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+    if (t1 > 0) stage(0);
+    __syncthreads();
+    for (int t = 0; t < t1; ++t) {
+        const unsigned char* K = lds + (t & 1) * BUF;
+        const unsigned char* V = K + tile_t::BYTES;
+        if (t + 1 < t1) fetch(t + 1);
+#pragma unroll
+        for (int r0 = 0; r0 < KT; r0 += 32) {
+            const int k0 = t * KT + r0;
+            if (k0 >= wend) break;
+            f32x16 s, p;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = p[e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                Frag<NP> k, v;
+                frag_rows<NP, DT, KT>(K, r0, i, k);
+                mma(s, k, q[i]);
+                frag_rows<NP, DT, KT>(V, r0, i, v);
+                mma(p, v, g[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f.sl2, -lse)) * (p[e] - delta);
+            if (k0 + 32 > wfull) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = k0 + acc_row(e) < vis ? s[e] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[8 * i + e];
+                Frag<NP> ds;
+                make_frag(x, ds);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<NP> k;
+                    frag_cols<NP, DT, KT>(K, r0 + 16 * i, 32 * d, k);
+                    mma(dq[d], k, ds);
+                }
+            }
+        }
+        if (t + 1 < t1) stage((t + 1) & 1);
+        __syncthreads();
+    }
+    if (!live || a.dq == nullptr) return;
+    T* dst = (T*)a.dq + b * a.dq_b + tq * a.dq_t + head * a.dq_h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = 32 * d + acc_row(e);
+            if (c < a.D) store4(dst + c, f32x4{dq[d][e], dq[d][e + 1], dq[d][e + 2], dq[d][e + 3]} * a.scale);
+        }
+}
+
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
+    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
+    typedef Tile<T, DT, QT, NT> tile_t;
+    constexpr int BUF = 2 * tile_t::BYTES + 2 * QT * 4;          // Q planes, dO planes, log-sums, deltas
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
+    const ctn_attn_args& a = f.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int off = a.Tk - a.Tq;
+    unsigned id = die_order(blockIdx.x, gridDim.x);
+    const int kt = id % f.nt;                                    // with a causal mask the first keys are seen most
+    id /= f.nt;
+    const int hk = id % a.Hk, b = id / a.Hk;
+    const int b0 = kt * 32 * NW, w0 = b0 + wave * 32, key = w0 + (lane & 31);
+
+    int len = a.Tk;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
+    const bool seen = key < len;
+    // query q sees key j when j <= q + off: block's and wave's first query, and the wave's first query without a mask
+    const int first = a.causal ? max(0, b0 - off) : 0, wfirst = a.causal ? max(0, w0 - off) : 0;
+    const int wfull = w0 + 32 > len ? a.Tq : a.causal ? w0 + 31 - off : 0;
+    const int t0 = first / QT;
+    const int nq = b0 < len && a.Tq > first ? (a.Tq + QT - 1) / QT - t0 : 0;      // query tiles per head
+    const int ntile = nq * f.G;
+
+    Frag<NP> k[KS], v[KS];
+    {
+        const T* kp = (const T*)a.k + b * a.k_b + key * a.k_t + hk * a.k_h;
+        const T* vp = (const T*)a.v + b * a.v_b + key * a.v_t + hk * a.v_h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * half;
+            Chunk<T> ck, cv;
+            if (seen && d < a.D) ck.load(kp + d), cv.load(vp + d);
+            else ck.zero(), cv.zero();
+            ck.frag(k[s]);
+            cv.frag(v[s]);
+        }
+    }
+
+    tile_t tq, tg;
+    constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
+    float stat[NS];
+    auto fetch = [&](const int i) {
+        const int head = hk * f.G + i / nq, q0 = (t0 + i % nq) * QT;
+        tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.q_t, a.Tq - q0, a.D);
+        tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.do_t, a.Tq - q0, a.D);
+#pragma unroll
+        for (int x = 0; x < NS; ++x) {
+            const int j = threadIdx.x + NT * x, r = q0 + j % QT;
+            const int64_t row = ((int64_t)b * a.H + head) * a.Tq + r;
+            if (j < QT) {
+                stat[x] = r < a.Tq ? a.lse[row] : INFINITY;
+                if (stat[x] == -INFINITY) stat[x] = INFINITY;    // sees nothing: every probability comes out as zero
+            } else if (j < 2 * QT) {
+                stat[x] = r < a.Tq ? f.delta[row] : 0.f;
+            }
+        }
+    };
+    auto stage = [&](const int buf) {
+        unsigned char* p = lds + buf * BUF;
+        tq.store(p);
+        tg.store(p + tile_t::BYTES);
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+            if (threadIdx.x + NT * x < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[threadIdx.x + NT * x] = stat[x];
+    };
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+    if (ntile > 0) {
+        fetch(0);
+        stage(0);
+    }
+    __syncthreads();
+    for (int i = 0; i < ntile; ++i) {
+        const unsigned char* Q = lds + (i & 1) * BUF;
+        const unsigned char* G = Q + tile_t::BYTES;
+        const float* st = reinterpret_cast<const float*>(G + tile_t::BYTES);
+        if (i + 1 < ntile) fetch(i + 1);
+#pragma unroll
+        for (int r0 = 0; r0 < QT; r0 += 32) {
+            const int q0 = (t0 + i % nq) * QT + r0;
+            if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
+            f32x16 s, p;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = p[e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                Frag<NP> x;
+                frag_rows<NP, DT, QT>(Q, r0, j, x);
+                mma(s, x, k[j]);
+                frag_rows<NP, DT, QT>(G, r0, j, x);
+                mma(p, x, v[j]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f32x4 lse = ctn_ld4(st + r0 + 8 * r + 4 * half), delta = ctn_ld4(st + QT + r0 + 8 * r + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * r + e], f.sl2, -lse[e]));
+                    s[4 * r + e] = w;
+                    p[4 * r + e] = w * (p[4 * r + e] - delta[e]);
+                }
+            }
+            if (q0 < wfull) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool on = seen && (!a.causal || key <= q0 + acc_row(e) + off);
+                    s[e] = on ? s[e] : 0.f;
+                    p[e] = on ? p[e] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x[8], y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[8 * j + e], y[e] = p[8 * j + e];
+                Frag<NP> w, ds;
+                make_frag(x, w);
+                make_frag(y, ds);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<NP> c;
+                    frag_cols<NP, DT, QT>(G, r0 + 16 * j, 32 * d, c);
+                    mma(dv[d], c, w);
+                    frag_cols<NP, DT, QT>(Q, r0 + 16 * j, 32 * d, c);
+                    mma(dk[d], c, ds);
+                }
+            }
+        }
+        if (i + 1 < ntile) stage((i + 1) & 1);
+        __syncthreads();
+    }
+    if (key >= a.Tk) return;
+    T* pk = (T*)a.dk + b * a.dk_b + key * a.dk_t + hk * a.dk_h;
+    T* pv = (T*)a.dv + b * a.dv_b + key * a.dv_t + hk * a.dv_h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = 32 * d + acc_row(e);
+            if (c >= a.D) continue;
+            if (a.dk) store4(pk + c, f32x4{dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]} * a.scale);
+            if (a.dv) store4(pv + c, f32x4{dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]});
+        }
+}
+
+int waves_for(const int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
+template <typename T, int DT>
+void launch_dq(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
+    if (nw == 1) hipLaunchKernelGGL((attn_dq_kernel<T, DT, 1>), dim3(grid), dim3(64), 0, s, f);
+    else if (nw == 2) hipLaunchKernelGGL((attn_dq_kernel<T, DT, 2>), dim3(grid), dim3(128), 0, s, f);
+    else hipLaunchKernelGGL((attn_dq_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
+}
+template <typename T, int DT>
+void launch_dkv(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
+    if (nw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 1>), dim3(grid), dim3(64), 0, s, f);
+    else if (nw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 2>), dim3(grid), dim3(128), 0, s, f);
+    else hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
+}
+template <typename T>
+void launch_bwd(const bool keys, const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
+    if (f.a.D <= 32) keys ? launch_dkv<T, 32>(f, nw, grid, s) : launch_dq<T, 32>(f, nw, grid, s);
+    else if (f.a.D <= 64) keys ? launch_dkv<T, 64>(f, nw, grid, s) : launch_dq<T, 64>(f, nw, grid, s);
+    else keys ? launch_dkv<T, 128>(f, nw, grid, s) : launch_dq<T, 128>(f, nw, grid, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ctn_attn_bwd_ws_floats(const ctn_attn_args* a) {
+    if (!ctn_attn_args_ok(a, "ctn_attn_bwd_ws_floats")) return -1;
+    return (int64_t)a->batch * a->H * a->Tq;
+}
+
+int ctn_attn_bwd(const ctn_attn_args* a, void* stream) {
+    if (!ctn_attn_args_ok(a, "ctn_attn_bwd")) return CTN_ERR_ARG;
+    if (a->batch == 0) return CTN_OK;
+    const int es = a->type == CTN_TYPE_F32 ? 4 : 2;
+    const int64_t nrow = (int64_t)a->batch * a->H * a->Tq;
+    CTN_REQUIRE(a->Tq == 0 || (a->d_o && a->lse && strides_ok(a->d_o, a->do_b, a->do_t, a->do_h, es)),
+                "ctn_attn_bwd: d_o (16-byte aligned, strides of whole 16 bytes) and lse are needed");
+    CTN_REQUIRE((!a->dq || strides_ok(a->dq, a->dq_b, a->dq_t, a->dq_h, es)) &&
+                    (!a->dk || strides_ok(a->dk, a->dk_b, a->dk_t, a->dk_h, es)) &&
+                    (!a->dv || strides_ok(a->dv, a->dv_b, a->dv_t, a->dv_h, es)),
+                "ctn_attn_bwd: dq, dk, dv must be 16-byte aligned with strides of whole 16 bytes");
+    CTN_REQUIRE(nrow == 0 || (a->ws && a->ws_floats >= nrow), "ctn_attn_bwd: workspace of %lld floats, %lld needed",
+                (long long)a->ws_floats, (long long)nrow);
+    bwd_params f;
+    f.a = *a;
+    f.G = a->H / a->Hk;
+    f.sl2 = a->scale * LOG2E;
+    f.delta = a->ws;
+    hipStream_t s = (hipStream_t)stream;
+    if (a->Tq > 0) {                       // also where dq itself is not wanted: the second launch reads the deltas
+        const int nw = waves_for(a->Tq);
+        f.nt = ctn_cdiv(a->Tq, 32 * nw);
+        const int64_t grid = (int64_t)a->batch * a->H * f.nt;
+        CTN_REQUIRE(grid < 0x7fffffff, "ctn_attn_bwd: too much work for one launch");
+        if (a->type == CTN_TYPE_F32) launch_bwd<float>(false, f, nw, (unsigned)grid, s);
+        else launch_bwd<__bf16>(false, f, nw, (unsigned)grid, s);
+        CTN_CHECK_LAUNCH("ctn_attn_bwd (queries)");
+    }
+    if (a->Tk > 0 && (a->dk || a->dv)) {
+        const int nw = waves_for(a->Tk);
+        f.nt = ctn_cdiv(a->Tk, 32 * nw);
+        const int64_t grid = (int64_t)a->batch * a->Hk * f.nt;
+        CTN_REQUIRE(grid < 0x7fffffff, "ctn_attn_bwd: too much work for one launch");
+        if (a->type == CTN_TYPE_F32) launch_bwd<float>(true, f, nw, (unsigned)grid, s);
+        else launch_bwd<__bf16>(true, f, nw, (unsigned)grid, s);
+        CTN_CHECK_LAUNCH("ctn_attn_bwd (keys)");
+    }
+    return CTN_OK;
+}
+
+}  // extern "C"

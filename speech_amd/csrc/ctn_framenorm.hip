@@ -1,0 +1,389 @@
+// Layer norm over the features of each frame (rows with the features contiguous), forward and backward, gfx950.
+//
+//   y  = (x - mean) rstd gamma + beta,   rstd = 1 / sqrt(var + eps)
+//   dx = rstd (u - mean(u) - xhat mean(u xhat)),  u = dy gamma,  xhat = (x - mean) rstd
+//   dgamma = sum_rows dy xhat,  dbeta = sum_rows dy
+//
+// Bound by its streams: forward reads x and writes y, backward reads x and dy and writes dx, each exactly once.  A row is
+// owned by G lanes (8 .. 64 of a wave for short rows, a block of 256 or 1024 for long ones) that keep it in registers, 16
+// bytes per lane and load, so the statistics cost no second read.  The mean is refined by the mean of the differences to
+// its first estimate and kept as a sum of two floats: with eps far below the features' own rounding a constant row
+// would otherwise come out as its mean's rounding error times 1 / sqrt(eps).
+// Statistics, products and the column sums are fp32 whatever the element type; 16-bit results are rounded once.
+// The parameters' gradients are reduced in a fixed order (same bits on every run): a block keeps the column sums of the
+// rows it walks in registers and stores them to the caller's workspace, a second launch adds the blocks' sums.
+#include "ctn_common.h"
+
+namespace {
+
+typedef __bf16 fbf16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct FVec;
+template <> struct FVec<float> { static constexpr int V = 4; typedef f32x4 type; };
+template <> struct FVec<__bf16> { static constexpr int V = 8; typedef fbf16x8 type; };
+
+// V elements at p, of which the first n exist (zero beyond).  Rows need not be 16-byte aligned: the loads are of
+// element alignment, which global memory serves.
+template <typename T>
+__device__ __forceinline__ void fload(const T* __restrict__ p, const int n, float (&v)[FVec<T>::V]) {
+    constexpr int V = FVec<T>::V;
+    if (n >= V) {
+        typename FVec<T>::type t;
+        __builtin_memcpy(&t, p, 16);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (float)t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void fstore(T* __restrict__ p, const int n, const float (&v)[FVec<T>::V]) {
+    constexpr int V = FVec<T>::V;
+    if (n >= V) {
+        typename FVec<T>::type t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = (T)v[i];
+        __builtin_memcpy(p, &t, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) p[i] = (T)v[i];
+    }
+}
+// V parameters at index c of a float or (wbf) bf16 array; null: the constant `fill`
+template <int V>
+__device__ __forceinline__ void fparam(const void* __restrict__ w, const bool wbf, const int c, const int n, const float fill,
+                                       float (&v)[V]) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fill;
+    } else if (wbf) {
+        typedef __bf16 wvec __attribute__((ext_vector_type(V)));
+        wvec t;
+        if (n >= V) __builtin_memcpy(&t, (const __bf16*)w + c, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = n >= V ? (float)t[i] : i < n ? (float)((const __bf16*)w)[c + i] : 0.f;
+    } else {
+        typedef float wvec __attribute__((ext_vector_type(V)));
+        wvec t;
+        if (n >= V) __builtin_memcpy(&t, (const float*)w + c, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = n >= V ? t[i] : i < n ? ((const float*)w)[c + i] : 0.f;
+    }
+}
+
+// sums of NS values over the G lanes that own a row; every lane gets them.  G > 64: through LDS, one barrier, the caller
+// alternates `buf` between two slots of NS * (G / 64) floats so that no second barrier is needed.
+template <int G, int NS>
+__device__ __forceinline__ void fsum(float (&v)[NS], float* buf) {
+    constexpr int W = G < 64 ? G : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[i] += __shfl_xor(v[i], o);
+    if constexpr (G > 64) {
+        constexpr int NW = G / 64;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) buf[i * NW + wave] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            float t = buf[i * NW + (lane & (NW - 1))];
+#pragma unroll
+            for (int o = NW / 2; o > 0; o >>= 1) t += __shfl_xor(t, o);
+            v[i] = t;
+        }
+    }
+}
+
+template <int G> constexpr int fthreads() { return G > 256 ? G : 256; }
+
+// stats: three planes of R floats: mean, what the mean's rounding left over, rstd
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(fthreads<G>()) void frame_norm_fwd_kernel(const T* __restrict__ x, const int64_t ldx,
+                                                                       const int64_t R, const int C,
+                                                                       const void* __restrict__ gamma,
+                                                                       const void* __restrict__ beta, const bool wbf,
+                                                                       const float eps, T* __restrict__ y, const int64_t ldy,
+                                                                       float* __restrict__ stats) {
+    constexpr int V = FVec<T>::V, RPB = fthreads<G>() / G;
+    __shared__ float red[2][2 * (G > 64 ? G / 64 : 1)];
+    const int g = threadIdx.x % G;
+    const float invC = 1.f / (float)C;
+    float ga[NV][V], be[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + g) * V;
+        fparam<V>(gamma, wbf, c, C - c, 1.f, ga[k]);
+        fparam<V>(beta, wbf, c, C - c, 0.f, be[k]);
+    }
+    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < R; rb += (int64_t)gridDim.x * RPB) {
+        const int64_t row = rb + threadIdx.x / G;
+        const bool live = row < R;                     // G > 64: one row per block, uniform
+        float v[NV][V];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * G + g) * V;
+            fload<T>(x + row * ldx + c, live ? C - c : 0, v[k]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] += v[k][i];
+        }
+        fsum<G, 1>(s, red[0]);
+        const float m0 = s[0] * invC;
+        float d[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool in = (k * G + g) * V + i < C;
+                v[k][i] = in ? v[k][i] - m0 : 0.f;
+                d[0] += v[k][i];
+                d[1] += v[k][i] * v[k][i];
+            }
+        fsum<G, 2>(d, red[1]);
+        const float dm = d[0] * invC;
+        const float var = fmaxf(d[1] * invC - dm * dm, 0.f);
+        const float rstd = 1.f / sqrtf(var + eps);
+        if (live) {
+            if (stats != nullptr && g == 0) {
+                const float m = m0 + dm;
+                stats[row] = m;
+                stats[R + row] = dm - (m - m0);
+                stats[2 * R + row] = rstd;
+            }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = (k * G + g) * V;
+                if (c >= C) continue;
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = (v[k][i] - dm) * rstd * ga[k][i] + be[k][i];
+                fstore<T>(y + row * ldy + c, C - c, o);
+            }
+        }
+    }
+}
+
+// part: [gridDim.x][2][C] column sums of dy xhat and dy over the block's rows; null: not formed
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* __restrict__ dy, const int64_t lddy,
+                                                                       const T* __restrict__ x, const int64_t ldx,
+                                                                       const int64_t R, const int C,
+                                                                       const void* __restrict__ gamma, const bool wbf,
+                                                                       const float* __restrict__ stats,
+                                                                       T* __restrict__ dx, const int64_t lddx,
+                                                                       float* __restrict__ part) {
+    constexpr int V = FVec<T>::V, NT = fthreads<G>(), RPB = NT / G;
+    constexpr int CW = G < 64 ? G : 64;                          // lanes of a wave that hold distinct columns
+    __shared__ float red[2][2 * (G > 64 ? G / 64 : 1)];
+    __shared__ float fold[G <= 64 ? (NT / 64) * CW * NV * V : 1];
+    const int g = threadIdx.x % G;
+    const float invC = 1.f / (float)C;
+    float ga[NV][V], dg[NV][V], db[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + g) * V;
+        fparam<V>(gamma, wbf, c, C - c, 1.f, ga[k]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) dg[k][i] = db[k][i] = 0.f;
+    }
+    int flip = 0;
+    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < R; rb += (int64_t)gridDim.x * RPB) {
+        const int64_t row = rb + threadIdx.x / G;
+        const bool live = row < R;
+        float xh[NV][V], u[NV][V];
+        float mean = 0.f, mlow = 0.f, rstd = 0.f;
+        if (live) mean = stats[row], mlow = stats[R + row], rstd = stats[2 * R + row];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * G + g) * V;
+            fload<T>(x + row * ldx + c, live ? C - c : 0, xh[k]);
+            fload<T>(dy + row * lddy + c, live ? C - c : 0, u[k]);
+        }
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool in = (k * G + g) * V + i < C;
+                xh[k][i] = in ? ((xh[k][i] - mean) - mlow) * rstd : 0.f;
+                dg[k][i] += u[k][i] * xh[k][i];
+                db[k][i] += u[k][i];
+                u[k][i] *= ga[k][i];
+                s[0] += u[k][i];
+                s[1] += u[k][i] * xh[k][i];
+            }
+        fsum<G, 2>(s, red[flip]);
+        flip ^= 1;
+        const float a = s[0] * invC, b = s[1] * invC;
+        if (live && dx != nullptr) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = (k * G + g) * V;
+                if (c >= C) continue;
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = rstd * (u[k][i] - a - xh[k][i] * b);
+                fstore<T>(dx + row * lddx + c, C - c, o);
+            }
+        }
+    }
+    if (part == nullptr) return;
+    float* out = part + (int64_t)blockIdx.x * 2 * C;
+    if constexpr (G <= 64) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float t = w == 0 ? dg[k][i] : db[k][i];
+#pragma unroll
+                    for (int o = 32; o >= G; o >>= 1) t += __shfl_xor(t, o);
+                    if (lane < G) fold[(wave * CW + lane) * NV * V + k * V + i] = t;
+                }
+            __syncthreads();
+            for (int c = threadIdx.x; c < C; c += NT) {
+                const int i = c % V, gg = (c / V) % G, k = c / (V * G);
+                float t = 0.f;
+                for (int q = 0; q < NT / 64; ++q) t += fold[(q * CW + gg) * NV * V + k * V + i];
+                out[w * C + c] = t;
+            }
+            __syncthreads();
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (k * G + g) * V + i;
+                if (c < C) out[c] = dg[k][i], out[C + c] = db[k][i];
+            }
+    }
+}
+
+// Sums of the blocks' column sums in a fixed order: 64 columns per block, 16 threads a column.
+__global__ __launch_bounds__(1024) void frame_norm_param_kernel(const float* __restrict__ part, const int nb, const int C,
+                                                                void* __restrict__ dgamma, void* __restrict__ dbeta,
+                                                                const bool wbf) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, p = threadIdx.x >> 6;
+    const int col = blockIdx.x * 64 + lane;                       // of the 2 C columns
+    float t = 0.f;
+    if (col < 2 * C)
+#pragma unroll 8
+        for (int b = p; b < nb; b += 16) t += part[(int64_t)b * 2 * C + col];
+    red[p][lane] = t;
+    __syncthreads();
+    if (p == 0 && col < 2 * C) {
+#pragma unroll
+        for (int q = 1; q < 16; ++q) t += red[q][lane];
+        void* out = col < C ? dgamma : dbeta;
+        if (out != nullptr) {
+            const int c = col < C ? col : col - C;
+            if (wbf) ((__bf16*)out)[c] = (__bf16)t;
+            else ((float*)out)[c] = t;
+        }
+    }
+}
+
+// rows per block of the variant that takes rows of C elements of V per 16 bytes
+int frame_rpb(const int C, const int V) {
+    const int n = ctn_cdiv(C, V);
+    return n <= 8 ? 32 : n <= 16 ? 16 : n <= 32 ? 8 : n <= 128 ? 4 : 1;
+}
+// blocks of the backward pass: up to four of 256 threads a CU, at least 16 row groups each so that the column sums'
+// stores stay below a twentieth of the rows' own traffic
+int frame_bwd_blocks(const int64_t R, const int C, const int V) {
+    const int64_t groups = (R + frame_rpb(C, V) - 1) / frame_rpb(C, V);
+    int64_t nb = (groups + 15) / 16;
+    if (nb < 256) nb = groups < 256 ? groups : 256;
+    return (int)(nb > 1024 ? 1024 : nb);
+}
+
+constexpr int FRAME_MAX_C = 16384;     // 1024 lanes, 16 elements each
+
+#define FRAME_DISPATCH(T, LAUNCH)                                                                   \
+    do {                                                                                            \
+        const int n_ = ctn_cdiv(C, FVec<T>::V);                                                     \
+        if (n_ <= 8) LAUNCH(T, 8, 1);                                                               \
+        else if (n_ <= 16) LAUNCH(T, 16, 1);                                                        \
+        else if (n_ <= 32) LAUNCH(T, 32, 1);                                                        \
+        else if (n_ <= 64) LAUNCH(T, 64, 1);                                                        \
+        else if (n_ <= 128) LAUNCH(T, 64, 2);                                                       \
+        else if (n_ <= 256) LAUNCH(T, 256, 1);                                                      \
+        else if (n_ <= 512) LAUNCH(T, 256, 2);                                                      \
+        else if (n_ <= 1024) LAUNCH(T, 256, 4);                                                     \
+        else if (n_ <= 2048) LAUNCH(T, 1024, 2);                                                    \
+        else if constexpr (FVec<T>::V == 4) LAUNCH(T, 1024, 4);                                     \
+    } while (0)
+
+bool frame_type_ok(const int type) { return type == CTN_TYPE_F32 || type == CTN_TYPE_BF16; }
+
+}  // namespace
+
+extern "C" {
+
+int ctn_frame_norm_fwd(const void* x, int64_t ldx, int64_t R, int C, int type, const void* gamma, const void* beta, int wtype,
+                       float eps, void* y, int64_t ldy, float* stats, void* stream) {
+    CTN_REQUIRE(frame_type_ok(type) && (wtype == CTN_TYPE_F32 || wtype == type), "ctn_frame_norm_fwd: types %d / %d", type, wtype);
+    CTN_REQUIRE(R >= 0 && C > 0 && C <= FRAME_MAX_C, "ctn_frame_norm_fwd: R %lld, C %d (1 to %d features)", (long long)R, C,
+                FRAME_MAX_C);
+    if (R == 0) return CTN_OK;
+    CTN_REQUIRE(x && y && ldx >= 0 && ldy >= C && eps >= 0.f, "ctn_frame_norm_fwd: bad arguments");
+    const int V = type == CTN_TYPE_F32 ? 4 : 8;
+    const int64_t groups = (R + frame_rpb(C, V) - 1) / frame_rpb(C, V);
+    const unsigned grid = (unsigned)(groups < 2048 ? groups : 2048);      // eight blocks of 256 threads a CU; the parameters stay in registers
+    const bool wbf = wtype == CTN_TYPE_BF16;
+#define FRAME_FWD(T, G, NV)                                                                                                   \
+    hipLaunchKernelGGL((frame_norm_fwd_kernel<T, G, NV>), dim3(grid), dim3(fthreads<G>()), 0, (hipStream_t)stream, (const T*)x, \
+                       ldx, R, C, gamma, beta, wbf, eps, (T*)y, ldy, stats)
+    if (type == CTN_TYPE_F32) FRAME_DISPATCH(float, FRAME_FWD);
+    else FRAME_DISPATCH(__bf16, FRAME_FWD);
+#undef FRAME_FWD
+    CTN_CHECK_LAUNCH("ctn_frame_norm_fwd");
+    return CTN_OK;
+}
+
+int64_t ctn_frame_norm_bwd_ws_floats(int64_t R, int C, int type) {
+    if (!frame_type_ok(type) || R <= 0 || C <= 0 || C > FRAME_MAX_C) return 0;
+    return (int64_t)frame_bwd_blocks(R, C, type == CTN_TYPE_F32 ? 4 : 8) * 2 * C;
+}
+
+int ctn_frame_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, int type,
+                       const void* gamma, int wtype, const float* stats, void* dx, int64_t lddx, void* dgamma, void* dbeta,
+                       float* ws, int64_t ws_floats, void* stream) {
+    CTN_REQUIRE(frame_type_ok(type) && (wtype == CTN_TYPE_F32 || wtype == type), "ctn_frame_norm_bwd: types %d / %d", type, wtype);
+    CTN_REQUIRE(R >= 0 && C > 0 && C <= FRAME_MAX_C, "ctn_frame_norm_bwd: R %lld, C %d (1 to %d features)", (long long)R, C,
+                FRAME_MAX_C);
+    CTN_REQUIRE(R == 0 || (dy && x && stats && lddy >= 0 && ldx >= 0 && (!dx || lddx >= C)), "ctn_frame_norm_bwd: bad arguments");
+    const bool params = dgamma != nullptr || dbeta != nullptr;
+    const int V = type == CTN_TYPE_F32 ? 4 : 8;
+    const int nb = R > 0 ? frame_bwd_blocks(R, C, V) : 0;
+    CTN_REQUIRE(!params || nb == 0 || (ws && ws_floats >= (int64_t)nb * 2 * C),
+                "ctn_frame_norm_bwd: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)nb * 2 * C);
+    const bool wbf = wtype == CTN_TYPE_BF16;
+    float* part = params ? ws : nullptr;
+    if (nb > 0) {
+#define FRAME_BWD(T, G, NV)                                                                                                    \
+    hipLaunchKernelGGL((frame_norm_bwd_kernel<T, G, NV>), dim3(nb), dim3(fthreads<G>()), 0, (hipStream_t)stream, (const T*)dy, \
+                       lddy, (const T*)x, ldx, R, C, gamma, wbf, stats, (T*)dx, lddx, part)
+        if (type == CTN_TYPE_F32) FRAME_DISPATCH(float, FRAME_BWD);
+        else FRAME_DISPATCH(__bf16, FRAME_BWD);
+#undef FRAME_BWD
+        CTN_CHECK_LAUNCH("ctn_frame_norm_bwd");
+    }
+    if (params) {
+        hipLaunchKernelGGL(frame_norm_param_kernel, dim3(ctn_cdiv(2 * (int64_t)C, 64)), dim3(1024), 0, (hipStream_t)stream, part, nb, C,
+                           dgamma, dbeta, wbf);
+        CTN_CHECK_LAUNCH("ctn_frame_norm_bwd (parameters)");
+    }
+    return CTN_OK;
+}
+
+}  // extern "C"

@@ -588,6 +588,74 @@ class LstmFn(torch.autograd.Function):
         return (dx, None) + tuple(grads)
 
 
+# ------------------------------------------------------------------------------------------------ frame norm, rotary positions, attention
+class FrameNormFn(torch.autograd.Function):
+    """Layer norm over the last axis of x (..., C), parameters (C,) in fp32 or x's type (None: not applied)."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps):
+        ops._require_cuda(x)
+        x2 = ops.feature_rows(x.detach())
+        needs = any(ctx.needs_input_grad[:3])
+        y, stats = ops.frame_norm_fwd(x2, None if gamma is None else gamma.detach().contiguous(),
+                                      None if beta is None else beta.detach().contiguous(), eps, want_stats=needs)
+        if needs:
+            ctx.save_for_backward(x, gamma, stats)
+            ctx.beta_dtype = None if beta is None else beta.dtype
+        return y.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gamma, stats = ctx.saved_tensors
+        dx, dgamma, dbeta = ops.frame_norm_bwd(
+            ops.feature_rows(dy), ops.feature_rows(x), None if gamma is None else gamma.contiguous(), stats,
+            ctx.needs_input_grad[0], gamma.dtype if ctx.needs_input_grad[1] else None,
+            ctx.beta_dtype if ctx.needs_input_grad[2] else None)
+        return None if dx is None else dx.view(x.shape), dgamma, dbeta, None
+
+
+class RotaryFn(torch.autograd.Function):
+    """x (B, T, H, D) with its heads' leading pairs rotated by their positions; the gradient is turned back."""
+
+    @staticmethod
+    def forward(ctx, x, turns, positions, first, interleaved, magnitude):
+        ops._require_cuda(x)
+        ctx.meta = (first, interleaved, magnitude)
+        ctx.save_for_backward(turns, positions)
+        return ops.rotary(x.detach(), turns, positions, first, interleaved, False, magnitude)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        turns, positions = ctx.saved_tensors
+        first, interleaved, magnitude = ctx.meta
+        return ops.rotary(dy, turns, positions, first, interleaved, True, magnitude), None, None, None, None, None
+
+
+class AttentionFn(torch.autograd.Function):
+    """softmax(scale q k^T) v over the visible keys, q (B, Tq, H, D), k and v (B, Tk, Hk, D); the backward pass forms the
+    probabilities again from the forward pass's log-sums."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, causal, scale):
+        ops._require_cuda(q, k, v)
+        needs = any(ctx.needs_input_grad[:3])
+        o, lse = ops.attn_fwd(q.detach(), k.detach(), v.detach(), lengths, causal, scale, want_lse=needs)
+        if needs:
+            ctx.save_for_backward(q, k, v, o, lse, lengths)
+            ctx.meta = (causal, scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        causal, scale = ctx.meta
+        dq, dk, dv = ops.attn_bwd(do, q, k, v, o, lse, lengths, causal, scale, ctx.needs_input_grad[:3])
+        return dq, dk, dv, None, None, None
+
+
 # ------------------------------------------------------------------------------------------------ axis shuffles of the dual-path blocks
 class RowsFromBlocksFn(torch.autograd.Function):
     """(B, F, S, K) -> the recurrence's rows (B*S, K, F) (walk_chunks False) or (B*K, S, F) (True), i.e.

@@ -1,0 +1,122 @@
+"""Attention over the frames of a sequence, with rotary positions: what the dual-path blocks' attention form
+(models/dprnn.py) puts in the place of the recurrence (src/models/dprnn.py:60-64, :104-114 of the reference).  Tensors are
+(batch, tokens, heads, features); the kernels are ctn_attn_fwd / ctn_attn_bwd and ctn_rotary."""
+import math
+
+import torch
+import torch.nn as nn
+
+from ..functional import AttentionFn, LinearFn, RotaryFn
+
+
+def attention(q, k, v, lengths=None, causal=False, scale=None):
+    """softmax(scale * q k^T) v over the visible keys, head by head, with gradients for q, k and v.
+
+    Key j is visible to query i when j < lengths[b] and, if causal, j <= i + Tk - Tq: the last query sees the last key, so a
+    few new queries against all keys so far need no other mask.  A row that sees no key is zero.  Keys and values behind a
+    sequence's length are never read.
+
+    Args:
+        q (B, Tq, H, D), k and v (B, Tk, Hk, D): float32 or bfloat16, H a multiple of Hk (query heads of a key head are
+            adjacent), D a multiple of 8 up to 128; any strides (views of a fused projection are taken as they are)
+        lengths (B,): whole numbers on the tensors' device, or None
+        scale: positive number, None for 1 / sqrt(D)
+    Returns:
+        output (B, Tq, H, D), dense
+    """
+    return AttentionFn.apply(q, k, v, lengths, bool(causal), scale)
+
+
+def rotate(input, turns, positions=None, offset=0, interleaved=False, magnitude=1.0):
+    """input (B, T, H, D) with the leading 2 * len(turns) features of every head rotated pair by pair by
+    2 pi * position * turns[pair] and scaled by `magnitude`; differentiable in input.
+
+    Args:
+        turns: float64 on the input's device, turns per position of each pair (RotaryPositions makes them)
+        positions: whole numbers (T,) or (B, T) on the input's device; None: offset, offset + 1, ...
+        interleaved: pairs (2 i, 2 i + 1) instead of (i, i + len(turns))
+    """
+    return RotaryFn.apply(input, turns, positions, int(offset), bool(interleaved), float(magnitude))
+
+
+def rotary_turns(rotary_dim, base=10000.0, scaling=None):
+    """Turns per position of the rotary_dim / 2 pairs, base^(-2 i / rotary_dim) / (2 pi), and the factor for the rotated
+    features.  scaling, for contexts longer than the one trained on:
+        None
+        ('linear', factor)                 every position divided by factor
+        ('base', factor)                   base * factor^(rotary_dim / (rotary_dim - 2)): the slowest pair is slowed by
+                                           factor, the fastest not at all
+        ('ramp', factor, length, low, high)    pairs that make fewer than `low` turns over `length` positions are slowed by
+                                           factor, those above `high` not, linear in between; the rotated features are
+                                           scaled by 0.1 ln(factor) + 1
+    """
+    if rotary_dim % 2 or rotary_dim < 0:
+        raise ValueError("rotary_dim is expected to be an even number, but given {}".format(rotary_dim))
+    kind = None if scaling is None else scaling[0]
+    if kind not in (None, 'linear', 'base', 'ramp') or (scaling is not None and not scaling[1] >= 1):
+        raise ValueError("Not support rotary scaling {}.".format(scaling))
+    if kind == 'base':
+        if rotary_dim <= 2:
+            raise ValueError("'base' scaling needs more than one pair")
+        base = base * scaling[1] ** (rotary_dim / (rotary_dim - 2))
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    turns = base ** (-i / max(rotary_dim, 1)) / (2 * math.pi)
+    magnitude = 1.0
+    if kind == 'linear':
+        turns = turns / scaling[1]
+    elif kind == 'ramp':
+        _, factor, length, low, high = scaling
+        if not low < high:
+            raise ValueError("'ramp' scaling needs low < high, but given {} and {}".format(low, high))
+        keep = ((turns * length - low) / (high - low)).clamp(0, 1)
+        turns = turns * (keep + (1 - keep) / factor)
+        magnitude = 0.1 * math.log(factor) + 1
+    return turns, magnitude
+
+
+class RotaryPositions(nn.Module):
+    """Rotary positions for heads of `head_dim` features: forward(x, positions=None, offset=0) rotates x (B, T, H, D).
+    rotary_dim: how many leading features of a head turn (default: all).  No parameters; the frequencies are kept in
+    float64 through every cast of the module (as the bits of whole numbers) and are not part of its state_dict."""
+
+    def __init__(self, head_dim, rotary_dim=None, base=10000.0, interleaved=False, scaling=None):
+        super().__init__()
+        self.head_dim = head_dim
+        self.rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if self.rotary_dim > head_dim:
+            raise ValueError("rotary_dim is expected to be at most {}, but given {}".format(head_dim, rotary_dim))
+        self.interleaved = interleaved
+        turns, self.magnitude = rotary_turns(self.rotary_dim, base, scaling)
+        self.register_buffer('turns_bits', turns.view(torch.int64), persistent=False)
+
+    @property
+    def turns(self):
+        return self.turns_bits.view(torch.float64)
+
+    def forward(self, input, positions=None, offset=0):
+        if input.size(-1) != self.head_dim:
+            raise ValueError("heads of {} features expected, got {}".format(self.head_dim, input.size(-1)))
+        return rotate(input, self.turns, positions, offset, self.interleaved, self.magnitude)
+
+
+class SelfAttention(nn.Module):
+    """Multi-head self-attention with rotary positions, up to (not including) its output projection:
+    (N, T, num_features) -> (N, T, hidden_channels), as an RNN layer of that output size would."""
+
+    def __init__(self, num_features, hidden_channels, num_heads=4, causal=False):
+        super().__init__()
+        if hidden_channels % num_heads or (hidden_channels // num_heads) % 8 or hidden_channels // num_heads > 128:
+            raise ValueError("hidden_channels is expected to be num_heads times a multiple of 8 up to 128, but given {} and "
+                             "{} heads".format(hidden_channels, num_heads))
+        self.num_heads, self.head_dim = num_heads, hidden_channels // num_heads
+        self.causal = causal
+        self.in_proj = nn.Linear(num_features, 3 * hidden_channels)
+        self.rotary = RotaryPositions(self.head_dim)
+
+    def forward(self, input, lengths=None):
+        N, T, _ = input.size()
+        H, D = self.num_heads, self.head_dim
+        qkv = LinearFn.apply(input, self.in_proj.weight, self.in_proj.bias).view(N, T, 3 * H, D)
+        qk = self.rotary(qkv[:, :, :2 * H])
+        out = attention(qk[:, :, :H], qk[:, :, H:], qkv[:, :, 2 * H:], lengths=lengths, causal=self.causal)
+        return out.view(N, T, H * D)

@@ -1,9 +1,10 @@
 """Layer norms with the reference's interface and state_dict keys (src/modules/norm.py), running on the
-HIP statistics / apply kernels (ctn_norm_*)."""
+HIP statistics / apply kernels (ctn_norm_*), and the norm over the features of each frame (ctn_frame_norm_*), which the
+reference does not have."""
 import torch
 import torch.nn as nn
 
-from ..functional import LayerNormFn
+from ..functional import FrameNormFn, LayerNormFn
 
 EPS = 1e-12
 
@@ -59,6 +60,44 @@ class CumulativeLayerNorm1d(nn.Module):
         if input.dim() not in (3, 4):
             raise ValueError("Only support 3D or 4D input, but given {}D".format(input.dim()))
         return LayerNormFn.apply(input, self.gamma, self.beta, self.eps, True)
+
+    def __repr__(self):
+        return '{}({}, eps={})'.format(self.__class__.__name__, self.num_features, self.eps)
+
+
+def frame_layer_norm(input, weight=None, bias=None, eps=EPS):
+    """Layer norm over the last axis: (input - mean) / sqrt(var + eps) * weight + bias.
+
+    Args:
+        input (..., C), float32 or bfloat16, C up to 16384
+        weight, bias (C,) in float32 or the input's type, or None
+    Returns:
+        output: same shape and type as the input (dense)
+    """
+    if input.dim() < 1 or input.size(-1) < 1:
+        raise ValueError("frame_layer_norm needs at least one feature, got {}".format(tuple(input.shape)))
+    return FrameNormFn.apply(input, weight, bias, eps)
+
+
+class FrameLayerNorm(nn.Module):
+    """Layer normalization over the features of each frame, features last: every frame on its own, so causal by
+    construction, and on rows as the dual-path blocks lay them out."""
+
+    def __init__(self, num_features, eps=EPS):
+        super().__init__()
+        self.num_features = num_features
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features))
+
+    def forward(self, input):
+        """
+        Args:
+            input (..., num_features)
+        Returns:
+            output: same shape as the input
+        """
+        return frame_layer_norm(input, self.weight, self.bias, self.eps)
 
     def __repr__(self):
         return '{}({}, eps={})'.format(self.__class__.__name__, self.num_features, self.eps)

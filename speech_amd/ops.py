@@ -360,6 +360,207 @@ def rows_wgrad(dy, x, dW=None, dbias=None, sign=1.0, arith=None):
 
 
 # ------------------------------------------------------------------------------------------------ axis shuffles
+# ------------------------------------------------------------------------------------------------ frame norm, rotary positions, attention
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
+FRAME_NORM_MAX_FEATURES = 16384
+ATTENTION_MAX_HEAD = 128
+
+
+def _type(t, what):
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise _lib.CtnError("{}: float32 or bfloat16 tensors, got {}".format(what, t.dtype))
+    return code
+
+
+def _same_place(what, first, *rest):
+    _require_cuda(first, *rest)
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise _lib.CtnError("{}: tensors on {} and {}".format(what, first.device, t.device))
+
+
+def _enqueue(name, t, fn, *args):
+    """fn(*args, stream) on the current stream of t's device, which need not be the current device."""
+    if t.device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+        return
+    with torch.cuda.device(t.device):
+        _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def feature_rows(x):
+    """(..., C) as (rows, C) with unit feature stride: a view where the strides allow it."""
+    x2 = x.reshape(-1, x.shape[-1])
+    return x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous()
+
+
+def frame_norm_fwd(x2, gamma, beta, eps, want_stats=True):
+    """x2 (R, C) rows -> y (R, C), stats (3, R) for frame_norm_bwd (None unless wanted); see ctn_frame_norm_fwd."""
+    lib = _lib.load()
+    _same_place("frame_norm", x2, gamma, beta)
+    R, Cc = x2.shape
+    code = _type(x2, "frame_norm")
+    wcode = code
+    for w in (gamma, beta):
+        if w is None:
+            continue
+        if w.numel() != Cc or not w.is_contiguous():
+            raise _lib.CtnError("frame_norm: parameters of {} contiguous elements, got {}".format(Cc, tuple(w.shape)))
+        wcode = _type(w, "frame_norm")
+    if (gamma is not None and beta is not None and gamma.dtype != beta.dtype) or wcode not in (_lib.TYPE_F32, code):
+        raise _lib.CtnError("frame_norm: parameters in float32 or the input's type, both alike")
+    y = torch.empty((R, Cc), device=x2.device, dtype=x2.dtype)
+    stats = torch.empty((3, R), device=x2.device, dtype=torch.float32) if want_stats else None
+    _enqueue("ctn_frame_norm_fwd", x2, lib.ctn_frame_norm_fwd, _ptr(x2), _ld(x2), R, Cc, code, _ptr(gamma), _ptr(beta), wcode,
+             float(eps), _ptr(y), Cc, _ptr(stats))
+    return y, stats
+
+
+def frame_norm_bwd(dy2, x2, gamma, stats, want_dx=True, want_dgamma=None, want_dbeta=None):
+    """-> dx (R, C), dgamma (C,), dbeta (C,), each None unless wanted (want_dgamma / want_dbeta: the parameter's dtype);
+    see ctn_frame_norm_bwd."""
+    lib = _lib.load()
+    _same_place("frame_norm", x2, dy2, gamma, stats)
+    R, Cc = x2.shape
+    code = _type(x2, "frame_norm")
+    assert dy2.shape == x2.shape and dy2.dtype == x2.dtype
+    dev = x2.device
+    wdtype = want_dgamma or want_dbeta or (torch.float32 if gamma is None else gamma.dtype)
+    dx = torch.empty((R, Cc), device=dev, dtype=x2.dtype) if want_dx else None
+    dgamma = torch.empty((Cc,), device=dev, dtype=wdtype) if want_dgamma else None
+    dbeta = torch.empty((Cc,), device=dev, dtype=wdtype) if want_dbeta else None
+    need = lib.ctn_frame_norm_bwd_ws_floats(R, Cc, code) if want_dgamma or want_dbeta else 0
+    ws = torch.empty((need,), device=dev, dtype=torch.float32) if need else None
+    _enqueue("ctn_frame_norm_bwd", x2, lib.ctn_frame_norm_bwd, _ptr(dy2), _ld(dy2), _ptr(x2), _ld(x2), R, Cc, code,
+             _ptr(gamma), _TYPES[wdtype], _ptr(stats), _ptr(dx), Cc, _ptr(dgamma), _ptr(dbeta), _ptr(ws), need)
+    return dx, dgamma, dbeta
+
+
+def _unit_last(x):
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, magnitude=1.0):
+    """x (B, T, H, D) with its leading 2 * turns.numel() elements per head rotated -> dense (B, T, H, D); see ctn_rotary.
+    turns: float64 on x's device; positions: int64 (T,) or (B, T), None: first, first + 1, ..."""
+    lib = _lib.load()
+    _same_place("rotary", x, turns, positions)
+    code = _type(x, "rotary")
+    if x.dim() != 4:
+        raise _lib.CtnError("rotary: a (batch, tokens, heads, features) tensor, got {} dimensions".format(x.dim()))
+    B, T, H, D = x.shape
+    if turns.dtype != torch.float64 or turns.dim() != 1 or 2 * turns.numel() > D:
+        raise _lib.CtnError("rotary: turns in float64, at most {} of them for {} features".format(D // 2, D))
+    turns = turns.contiguous()
+    pbs = 0
+    if positions is not None:
+        if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) not in ((T,), (B, T)):
+            raise _lib.CtnError("rotary: whole positions of shape ({},) or ({}, {}), got {} {}".format(
+                T, B, T, positions.dtype, tuple(positions.shape)))
+        positions = positions.to(torch.int64).contiguous()
+        pbs = T if positions.dim() == 2 else 0
+    x = _unit_last(x)
+    y = torch.empty((B, T, H, D), device=x.device, dtype=x.dtype)
+    _enqueue("ctn_rotary", x, lib.ctn_rotary, _ptr(x), x.stride(0), x.stride(1), x.stride(2), B, T, H, D, code,
+             _ptr(positions), pbs, int(first), _ptr(turns), 2 * turns.numel(), 1 if interleaved else 0, 1 if inverse else 0,
+             float(magnitude), _ptr(y), y.stride(0), y.stride(1), y.stride(2))
+    return y
+
+
+def _attn_operand(x):
+    """x with unit feature stride, 16-byte aligned, all strides whole 16 bytes: itself or a dense copy."""
+    per = 16 // x.element_size()
+    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(x.stride(i) % per == 0 or x.shape[i] == 1 for i in range(3)):
+        return x
+    return x.contiguous()
+
+
+def _attn_strides(x):
+    return tuple(0 if x.shape[i] == 1 else x.stride(i) for i in range(3))
+
+
+def _attn_args(q, k, v, o, lse, lengths, causal, scale):
+    B, Tq, H, D = q.shape
+    a = _lib.AttnArgs()
+    a.batch, a.Tq, a.Tk, a.H, a.Hk, a.D = B, Tq, k.shape[1], H, k.shape[2], D
+    a.type, a.causal, a.scale = _TYPES[q.dtype], 1 if causal else 0, scale
+    a.lengths = _ptr(lengths)
+    a.q, a.k, a.v, a.o, a.lse = _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse)
+    a.q_b, a.q_t, a.q_h = _attn_strides(q)
+    a.k_b, a.k_t, a.k_h = _attn_strides(k)
+    a.v_b, a.v_t, a.v_h = _attn_strides(v)
+    a.o_b, a.o_t, a.o_h = _attn_strides(o)
+    return a
+
+
+def check_attention(q, k, v, lengths):
+    """Raises CtnError unless attn_fwd takes these tensors."""
+    _same_place("attention", q, k, v, lengths)
+    code = _type(q, "attention")
+    if any(t.dim() != 4 for t in (q, k, v)) or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise _lib.CtnError("attention: q (B, Tq, H, D), k and v (B, Tk, Hk, D), got {}, {}, {}".format(
+            tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if _TYPES.get(k.dtype) != code or _TYPES.get(v.dtype) != code:
+        raise _lib.CtnError("attention: q, k and v of one type, got {}, {}, {}".format(q.dtype, k.dtype, v.dtype))
+    H, Hk, D = q.shape[2], k.shape[2], q.shape[3]
+    if Hk < 1 or H < 1 or H % Hk:
+        raise _lib.CtnError("attention: {} query heads for {} key heads (a multiple)".format(H, Hk))
+    if D % 8 or not 8 <= D <= ATTENTION_MAX_HEAD:
+        raise _lib.CtnError("attention: {} features per head (multiples of 8 up to {})".format(D, ATTENTION_MAX_HEAD))
+    if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (q.shape[0],)):
+        raise _lib.CtnError("attention: whole lengths of shape ({},), got {} {}".format(
+            q.shape[0], lengths.dtype, tuple(lengths.shape)))
+
+
+def attn_fwd(q, k, v, lengths=None, causal=False, scale=None, want_lse=True):
+    """q (B, Tq, H, D), k, v (B, Tk, Hk, D) -> o dense like q, lse (B, H, Tq) fp32 (None unless wanted); see ctn_attn_fwd."""
+    lib = _lib.load()
+    check_attention(q, k, v, lengths)
+    B, Tq, H, D = q.shape
+    scale = D ** -0.5 if scale is None else float(scale)
+    q, k, v = _attn_operand(q), _attn_operand(k), _attn_operand(v)
+    if lengths is not None:
+        lengths = lengths.clamp(0, k.shape[1]).to(torch.int32) if lengths.dtype == torch.int64 else lengths
+        lengths = lengths.contiguous()
+    o = torch.empty((B, Tq, H, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((B, H, Tq), device=q.device, dtype=torch.float32) if want_lse else None
+    a = _attn_args(q, k, v, o, lse, lengths, causal, scale)
+    need = lib.ctn_attn_fwd_ws_floats(C.byref(a))
+    ws = torch.empty((need,), device=q.device, dtype=torch.float32) if need > 0 else None
+    a.ws, a.ws_floats = _ptr(ws), max(need, 0)
+    _enqueue("ctn_attn_fwd", q, lib.ctn_attn_fwd, C.byref(a))
+    return o, lse
+
+
+def attn_bwd(do, q, k, v, o, lse, lengths=None, causal=False, scale=None, want=(True, True, True)):
+    """-> dq, dk, dv (dense, each None unless wanted) from the gradient of o and what attn_fwd returned; see ctn_attn_bwd."""
+    lib = _lib.load()
+    check_attention(q, k, v, lengths)
+    _same_place("attention", q, do, o, lse)
+    assert do.shape == q.shape and do.dtype == q.dtype
+    B, Tq, H, D = q.shape
+    scale = D ** -0.5 if scale is None else float(scale)
+    q, k, v, do = _attn_operand(q), _attn_operand(k), _attn_operand(v), _attn_operand(do)
+    if lengths is not None:
+        lengths = lengths.clamp(0, k.shape[1]).to(torch.int32) if lengths.dtype == torch.int64 else lengths
+        lengths = lengths.contiguous()
+    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if w else None for t, w in zip((q, k, v), want))
+    a = _attn_args(q, k, v, o, lse, lengths, causal, scale)
+    a.d_o, (a.do_b, a.do_t, a.do_h) = _ptr(do), _attn_strides(do)
+    if dq is not None:
+        a.dq, (a.dq_b, a.dq_t, a.dq_h) = _ptr(dq), _attn_strides(dq)
+    if dk is not None:
+        a.dk, (a.dk_b, a.dk_t, a.dk_h) = _ptr(dk), _attn_strides(dk)
+    if dv is not None:
+        a.dv, (a.dv_b, a.dv_t, a.dv_h) = _ptr(dv), _attn_strides(dv)
+    need = lib.ctn_attn_bwd_ws_floats(C.byref(a))
+    ws = torch.empty((need,), device=q.device, dtype=torch.float32) if need > 0 else None
+    a.ws, a.ws_floats = _ptr(ws), max(need, 0)
+    _enqueue("ctn_attn_bwd", q, lib.ctn_attn_bwd, C.byref(a))
+    return dq, dk, dv
+
+
 def _reaches(t, last):
     """True if element offset `last` (from t's first element) lies inside t's storage."""
     return t.storage_offset() + last < t.untyped_storage().nbytes() // 4
