@@ -11,6 +11,9 @@ through speech_amd.functional.LstmFn) -- one launch per sequence walk instead of
 with the input projection of all steps and the weight gradients as single large GEMMs.  The norms are this package's
 kernels as well, and so are the axis shuffles between the two layouts (tiled transposes, ctn_permute); the linear layer
 is torch's (a plain library GEMM).
+
+rnn_type='attention', which the reference does not have, puts self-attention with rotary positions in the recurrence's place
+(`_PathAttention`): a layer norm over each frame's features in front, causal across chunks where the model is causal.
 """
 import warnings
 
@@ -19,6 +22,8 @@ import torch.nn as nn
 
 from .. import ops
 from ..functional import FeatureFirstFn, LinearFn, LstmFn, RowsFromBlocksFn, SwapAddFn
+from ..modules.attention import SelfAttention
+from ..modules.norm import FrameLayerNorm
 from ..utils.tasnet import choose_layer_norm
 
 EPS = 1e-12
@@ -109,11 +114,45 @@ class InterChunkRNN(_PathRNN):
                          norm_name='cLN' if causal else 'gLN', causal=causal, rnn_type=rnn_type, eps=eps)
 
 
+class _PathAttention(nn.Module):
+    """The same unit with self-attention along the axis: frame layer norm, multi-head attention with rotary positions over the
+    steps (hidden_channels features in num_heads heads), linear map back to the feature count, residual connection."""
+
+    def __init__(self, num_features, hidden_channels, walk_chunks, causal, norm, num_heads, eps):
+        super().__init__()
+        self.num_features, self.hidden_channels = num_features, hidden_channels
+        self.walk_chunks = walk_chunks
+        self.norm = norm
+        if norm:
+            self.norm1d = FrameLayerNorm(num_features, eps=eps)
+        self.attention = SelfAttention(num_features, hidden_channels, num_heads=num_heads, causal=causal)
+        self.fc = nn.Linear(hidden_channels, num_features)
+
+    def forward(self, input):
+        batch_size, num_features, S, K = input.size()
+        outer, steps = (K, S) if self.walk_chunks else (S, K)
+        y = RowsFromBlocksFn.apply(input, self.walk_chunks)                # (batch * outer, steps, features)
+        if self.norm:
+            y = self.norm1d(y)
+        y = LinearFn.apply(self.attention(y), self.fc.weight, self.fc.bias)
+        y = FeatureFirstFn.apply(y.view(batch_size, outer * steps, num_features))      # (batch, features, outer * steps)
+        y = y.view(batch_size, num_features, outer, steps)
+        if self.walk_chunks:
+            return SwapAddFn.apply(y, input)                               # back to (batch, features, S, K), plus input
+        return y + input
+
+
 class DPRNNBlock(nn.Module):
     """src/models/dprnn.py:30-48: the intra-chunk unit, then the inter-chunk unit."""
 
-    def __init__(self, num_features, hidden_channels, causal, norm=True, rnn_type='lstm', eps=EPS):
+    def __init__(self, num_features, hidden_channels, causal, norm=True, rnn_type='lstm', eps=EPS, num_heads=4):
         super().__init__()
+        if rnn_type == 'attention':
+            self.intra_chunk_block = _PathAttention(num_features, hidden_channels, walk_chunks=False, causal=False, norm=norm,
+                                                    num_heads=num_heads, eps=eps)
+            self.inter_chunk_block = _PathAttention(num_features, hidden_channels, walk_chunks=True, causal=causal, norm=norm,
+                                                    num_heads=num_heads, eps=eps)
+            return
         self.intra_chunk_block = IntraChunkRNN(num_features, hidden_channels, norm=norm, rnn_type=rnn_type, eps=eps)
         self.inter_chunk_block = InterChunkRNN(num_features, hidden_channels, causal=causal, norm=norm, rnn_type=rnn_type,
                                                eps=eps)
@@ -123,12 +162,14 @@ class DPRNNBlock(nn.Module):
 
 
 class DPRNN(nn.Module):
-    """src/models/dprnn.py:8-28: num_blocks dual-path blocks in sequence, (batch, features, S, K) in and out."""
+    """src/models/dprnn.py:8-28: num_blocks dual-path blocks in sequence, (batch, features, S, K) in and out.  num_heads: of
+    the attention form (rnn_type='attention')."""
 
-    def __init__(self, num_features, hidden_channels, num_blocks=6, norm=True, causal=False, rnn_type='lstm', eps=EPS):
+    def __init__(self, num_features, hidden_channels, num_blocks=6, norm=True, causal=False, rnn_type='lstm', eps=EPS,
+                 num_heads=4):
         super().__init__()
         self.net = nn.Sequential(*[DPRNNBlock(num_features, hidden_channels, causal=causal, norm=norm, rnn_type=rnn_type,
-                                              eps=eps) for _ in range(num_blocks)])
+                                              num_heads=num_heads, eps=eps) for _ in range(num_blocks)])
 
     def forward(self, input):
         return self.net(input)

@@ -2,7 +2,8 @@
 
 Encoder, decoder, the separator's entry norm, its two pointwise convolutions and the chunking / overlap-add with their
 paddings run on this package's HIP kernels, shared with Conv-TasNet; the dual-path blocks in between are described in
-models/dprnn.py; the PReLU, the mask non-linearity and the mask multiplication are torch tensor operations.
+models/dprnn.py (rnn_type='attention', sep_num_heads: their attention form); the PReLU, the mask non-linearity and the mask
+multiplication are torch tensor operations.
 """
 import torch
 import torch.nn as nn
@@ -49,6 +50,7 @@ class DPRNNTasNet(nn.Module):
         self.sep_norm = sep_norm
         self.mask_nonlinear = mask_nonlinear
         self.rnn_type = rnn_type
+        self.sep_num_heads = kwargs.pop('sep_num_heads', None) or 4        # of rnn_type='attention'
         self.n_sources = n_sources
         self.eps = eps
 
@@ -58,7 +60,8 @@ class DPRNNTasNet(nn.Module):
         self.separator = Separator(
             n_basis, bottleneck_channels=sep_bottleneck_channels, hidden_channels=sep_hidden_channels,
             chunk_size=sep_chunk_size, hop_size=sep_hop_size, num_blocks=sep_num_blocks, norm=sep_norm,
-            mask_nonlinear=mask_nonlinear, causal=causal, rnn_type=rnn_type, n_sources=n_sources, eps=eps)
+            mask_nonlinear=mask_nonlinear, causal=causal, rnn_type=rnn_type, n_sources=n_sources, eps=eps,
+            num_heads=self.sep_num_heads)
         self.decoder = decoder
 
     def forward(self, input):
@@ -99,6 +102,8 @@ class DPRNNTasNet(nn.Module):
             'n_sources': self.n_sources,
             'eps': self.eps
         }
+        if self.rnn_type == 'attention':
+            config['sep_num_heads'] = self.sep_num_heads
         return config
 
     @classmethod
@@ -117,7 +122,7 @@ class DPRNNTasNet(nn.Module):
             sep_chunk_size=config['sep_chunk_size'], sep_hop_size=config['sep_hop_size'],
             sep_num_blocks=config['sep_num_blocks'], sep_norm=config['sep_norm'], mask_nonlinear=config['mask_nonlinear'],
             causal=config['causal'], rnn_type=config.get('rnn_type', 'lstm'), n_sources=config['n_sources'],
-            eps=config.get('eps') or EPS)
+            eps=config.get('eps') or EPS, sep_num_heads=config.get('sep_num_heads'))
         if load_state_dict:
             model.load_state_dict(config['state_dict'])
         return model
@@ -136,7 +141,8 @@ class Separator(nn.Module):
     """src/models/dprnn_tasnet.py:288-350"""
 
     def __init__(self, num_features, bottleneck_channels=64, hidden_channels=128, chunk_size=100, hop_size=50,
-                 num_blocks=6, norm=True, mask_nonlinear='sigmoid', causal=True, rnn_type='lstm', n_sources=2, eps=EPS):
+                 num_blocks=6, norm=True, mask_nonlinear='sigmoid', causal=True, rnn_type='lstm', n_sources=2, eps=EPS,
+                 num_heads=4):
         super().__init__()
         self.num_features, self.n_sources = num_features, n_sources
         self.chunk_size, self.hop_size = chunk_size, hop_size
@@ -147,7 +153,7 @@ class Separator(nn.Module):
         self.bottleneck_conv1d = nn.Conv1d(num_features, bottleneck_channels, kernel_size=1, stride=1)
         self.segment1d = Segment1d(chunk_size, hop_size)
         self.dprnn = DPRNN(bottleneck_channels, hidden_channels, num_blocks=num_blocks, causal=causal, norm=norm,
-                           rnn_type=rnn_type, eps=eps)
+                           rnn_type=rnn_type, eps=eps, num_heads=num_heads)
         self.overlap_add1d = OverlapAdd1d(chunk_size, hop_size)
         self.prelu = nn.PReLU()
         self.mask_conv1d = nn.Conv1d(bottleneck_channels, n_sources * num_features, kernel_size=1, stride=1)

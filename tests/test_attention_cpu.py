@@ -170,3 +170,24 @@ def test_reference_gradients_against_differences():
     y = torch.nn.functional.layer_norm(leaves[0], (9,), leaves[1], leaves[2], 1e-6)
     for a, b in zip(out[1:], torch.autograd.grad(y, leaves, dy.double())):
         assert torch.allclose(a, b, rtol=1e-9, atol=1e-11)
+
+
+def test_dual_path_attention_model_config_and_keys(tmp_path):
+    from dprnn_cases import SMALL
+    from speech_amd.models.dprnn_tasnet import DPRNNTasNet
+    cfg = dict(SMALL, sep_hidden_channels=32, rnn_type='attention', sep_num_heads=2)
+    m = DPRNNTasNet(**cfg)
+    unit = m.separator.dprnn.net[0].inter_chunk_block
+    assert unit.attention.num_heads == 2 and unit.attention.causal is False
+    assert DPRNNTasNet(**dict(cfg, causal=True)).separator.dprnn.net[0].inter_chunk_block.attention.causal is True
+    assert DPRNNTasNet(**dict(cfg, causal=True)).separator.dprnn.net[0].intra_chunk_block.attention.causal is False
+    assert sorted(k for k in unit.state_dict()) == ["attention.in_proj.bias", "attention.in_proj.weight", "fc.bias", "fc.weight",
+                                                    "norm1d.bias", "norm1d.weight"]
+    path = str(tmp_path / "m.pth")
+    torch.save(dict(m.get_config(), state_dict=m.state_dict()), path)
+    b = DPRNNTasNet.build_model(path, load_state_dict=True)
+    assert b.get_config() == m.get_config() and b.sep_num_heads == 2
+    assert all(torch.equal(x, y) for x, y in zip(m.state_dict().values(), b.state_dict().values()))
+    assert "sep_num_heads" not in DPRNNTasNet(**SMALL).get_config()
+    with pytest.raises(NotImplementedError, match="Not support gru"):
+        DPRNNTasNet(**dict(SMALL, rnn_type='gru'))

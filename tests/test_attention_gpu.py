@@ -395,3 +395,70 @@ def test_calls_on_a_side_stream():
         got = [run_attention(q, k, v, do, None, False) for _ in range(3)]
     side.synchronize()
     assert all(torch.equal(a, b) for r in got for a, b in zip(r, base))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_dual_path_network_with_attention(causal):
+    """DPRNN-TasNet in its attention form: the separator's dual-path stack against the formula in 64 bits (through torch's own
+    operations on the CPU), gradients included; a causal stack's output does not depend on later chunks."""
+    from speech_amd.models.dprnn import DPRNN
+    torch.manual_seed(1)
+    net = DPRNN(16, 32, num_blocks=2, causal=causal, rnn_type='attention', num_heads=2).to(DEV)
+    x, dy = normal((2, 16, 7, 10), 1), normal((2, 16, 7, 10), 2)
+    xd = x.to(DEV).requires_grad_(True)
+    y = net(xd)
+    y.backward(dy.to(DEV))
+    params = {n: p.detach().cpu().double().requires_grad_(True) for n, p in net.named_parameters()}
+    x64 = x.double().requires_grad_(True)
+    turns, _ = rotary_turns(16)
+
+    def path(z, name, walk, mask):
+        P = {n: params[name + "." + n] for n in ("norm1d.weight", "norm1d.bias", "attention.in_proj.weight",
+                                                 "attention.in_proj.bias", "fc.weight", "fc.bias")}
+        r = z.permute(0, 3, 2, 1) if walk else z.permute(0, 2, 3, 1)
+        h = torch.nn.functional.layer_norm(r, (16,), P["norm1d.weight"], P["norm1d.bias"], 1e-12)
+        qkv = (h @ P["attention.in_proj.weight"].t() + P["attention.in_proj.bias"]).unflatten(-1, (6, 16))
+        T = r.shape[2]
+        ang = torch.arange(T).double()[:, None] * turns * 2 * math.pi
+        c, s = torch.cos(ang)[None, None, :, None], torch.sin(ang)[None, None, :, None]
+        a, b = qkv[..., :4, :8], qkv[..., :4, 8:]
+        qk = torch.cat((a * c - b * s, a * s + b * c), -1)
+        q, k, v = (t.transpose(2, 3) for t in (qk[..., :2, :], qk[..., 2:, :], qkv[..., 4:, :]))
+        sc = q @ k.transpose(-2, -1) / 4
+        if mask:
+            sc = sc.masked_fill(~torch.ones(T, T, dtype=torch.bool).tril(), -math.inf)
+        o = (torch.softmax(sc, -1) @ v).transpose(2, 3).flatten(-2) @ P["fc.weight"].t() + P["fc.bias"]
+        return z + (o.permute(0, 3, 2, 1) if walk else o.permute(0, 3, 1, 2))
+
+    z = x64
+    for i in range(2):
+        z = path(z, "net.%d.intra_chunk_block" % i, False, False)
+        z = path(z, "net.%d.inter_chunk_block" % i, True, causal)
+    z.backward(dy.double())
+
+    def rel(p, r):
+        return ((p.detach().cpu().double() - r).abs().max() / r.abs().max()).item()
+
+    assert rel(y, z.detach()) < 1e-4
+    assert rel(xd.grad, x64.grad) < 1e-4
+    for n, p in net.named_parameters():
+        assert rel(p.grad, params[n].grad) < 1e-4, n
+    if causal:
+        x2 = x.clone()
+        x2[:, :, 4:] += 1
+        with torch.no_grad():
+            assert torch.equal(net(x2.to(DEV))[:, :, :4], y.detach()[:, :, :4])
+
+
+def test_dual_path_tasnet_with_attention_trains_a_step():
+    from dprnn_cases import SMALL_CAUSAL3
+    from speech_amd.criterion.pit import PIT1d
+    from speech_amd.criterion.sdr import NegSISDR
+    from speech_amd.models.dprnn_tasnet import DPRNNTasNet
+    torch.manual_seed(1)
+    model = DPRNNTasNet(**dict(SMALL_CAUSAL3, sep_hidden_channels=32, rnn_type='attention')).to(DEV)
+    src = (0.1 * normal((2, 3, 250), 1)).to(DEV)
+    loss, _ = PIT1d(NegSISDR(), n_sources=3)(model(src.sum(1, keepdim=True)), src)
+    loss.backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in model.parameters())
+    assert all(p.grad.any() for n, p in model.named_parameters() if "in_proj.weight" in n)
