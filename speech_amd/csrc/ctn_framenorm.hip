@@ -25,17 +25,16 @@ template <> struct FVec<__bf16> { static constexpr int V = 8; typedef fbf16x8 ty
 // V elements at p, of which the first n exist (zero beyond).  Rows need not be 16-byte aligned: the loads are of
 // element alignment, which global memory serves.
 template <typename T>
-__device__ __forceinline__ void fload(const T* __restrict__ p, const int n, float (&v)[FVec<T>::V]) {
+__device__ __forceinline__ typename FVec<T>::type fload(const T* __restrict__ p, const int n) {
     constexpr int V = FVec<T>::V;
+    typename FVec<T>::type t;
     if (n >= V) {
-        typename FVec<T>::type t;
         __builtin_memcpy(&t, p, 16);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (float)t[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+        for (int i = 0; i < V; ++i) t[i] = i < n ? p[i] : (T)0.f;
     }
+    return t;
 }
 template <typename T>
 __device__ __forceinline__ void fstore(T* __restrict__ p, const int n, const float (&v)[FVec<T>::V]) {
@@ -120,18 +119,29 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_fwd_kernel(const T* 
         fparam<V>(gamma, wbf, c, C - c, 1.f, ga[k]);
         fparam<V>(beta, wbf, c, C - c, 0.f, be[k]);
     }
-    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < R; rb += (int64_t)gridDim.x * RPB) {
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    typename FVec<T>::type nx[NV];                     // the next row, in flight while this one is reduced
+    auto fetch = [&](const int64_t row) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * G + g) * V;
+            nx[k] = fload<T>(x + row * ldx + c, row < R ? C - c : 0);
+        }
+    };
+    fetch((int64_t)blockIdx.x * RPB + threadIdx.x / G);
+    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < R; rb += step) {
         const int64_t row = rb + threadIdx.x / G;
         const bool live = row < R;                     // G > 64: one row per block, uniform
         float v[NV][V];
         float s[1] = {0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * G + g) * V;
-            fload<T>(x + row * ldx + c, live ? C - c : 0, v[k]);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[0] += v[k][i];
-        }
+            for (int i = 0; i < V; ++i) {
+                v[k][i] = (float)nx[k][i];
+                s[0] += v[k][i];
+            }
+        fetch(row + step);
         fsum<G, 1>(s, red[0]);
         const float m0 = s[0] * invC;
         float d[2] = {0.f, 0.f};
@@ -192,18 +202,30 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* 
         for (int i = 0; i < V; ++i) dg[k][i] = db[k][i] = 0.f;
     }
     int flip = 0;
-    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < R; rb += (int64_t)gridDim.x * RPB) {
-        const int64_t row = rb + threadIdx.x / G;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    typename FVec<T>::type nx[NV], nd[NV];             // the next row, in flight while this one is reduced
+    float nm = 0.f, nl = 0.f, nr = 0.f;
+    auto fetch = [&](const int64_t row) {
         const bool live = row < R;
-        float xh[NV][V], u[NV][V];
-        float mean = 0.f, mlow = 0.f, rstd = 0.f;
-        if (live) mean = stats[row], mlow = stats[R + row], rstd = stats[2 * R + row];
+        nm = live ? stats[row] : 0.f, nl = live ? stats[R + row] : 0.f, nr = live ? stats[2 * R + row] : 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * G + g) * V;
-            fload<T>(x + row * ldx + c, live ? C - c : 0, xh[k]);
-            fload<T>(dy + row * lddy + c, live ? C - c : 0, u[k]);
+            nx[k] = fload<T>(x + row * ldx + c, live ? C - c : 0);
+            nd[k] = fload<T>(dy + row * lddy + c, live ? C - c : 0);
         }
+    };
+    fetch((int64_t)blockIdx.x * RPB + threadIdx.x / G);
+    for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < R; rb += step) {
+        const int64_t row = rb + threadIdx.x / G;
+        const bool live = row < R;
+        float xh[NV][V], u[NV][V];
+        const float mean = nm, mlow = nl, rstd = nr;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) xh[k][i] = (float)nx[k][i], u[k][i] = (float)nd[k][i];
+        fetch(row + step);
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k)

@@ -17,17 +17,16 @@ template <> struct XVec<float> { static constexpr int V = 4; typedef f32x4 type;
 template <> struct XVec<__bf16> { static constexpr int V = 8; typedef xbf16x8 type; };
 
 template <typename T>
-__device__ __forceinline__ void xload(const T* __restrict__ p, const int n, float (&v)[XVec<T>::V]) {
+__device__ __forceinline__ typename XVec<T>::type xload(const T* __restrict__ p, const int n) {
     constexpr int V = XVec<T>::V;
+    typename XVec<T>::type t;
     if (n >= V) {
-        typename XVec<T>::type t;
         __builtin_memcpy(&t, p, 16);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (float)t[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+        for (int i = 0; i < V; ++i) t[i] = i < n ? p[i] : (T)0.f;
     }
+    return t;
 }
 template <typename T>
 __device__ __forceinline__ void xstore(T* __restrict__ p, const int n, const float (&v)[XVec<T>::V]) {
@@ -92,31 +91,48 @@ __global__ __launch_bounds__(256) void rotary_kernel(const rotary_args a) {
                 cs[i] *= a.magnitude;
             }
         }
-        for (int h = h0; h < a.H; h += a.hs) {
-            const T* x = (const T*)a.x + b * a.xbs + t * a.xts + h * a.xhs + e0;
-            T* y = (T*)a.y + b * a.ybs + t * a.yts + h * a.yhs + e0;
-            float v[V], o[V];
-            xload<T>(x, ne, v);
-            if (!rot) {
-                xstore<T>(y, ne, v);
-            } else if (INTERLEAVED) {
+        // four heads at a time: their loads are in flight together
+        const T* x = (const T*)a.x + b * a.xbs + t * a.xts + e0;
+        T* y = (T*)a.y + b * a.ybs + t * a.yts + e0;
+        for (int hb = h0; hb < a.H; hb += 4 * a.hs) {
+            typename XVec<T>::type r[4], q[4];
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    o[2 * i] = v[2 * i] * cs[i] - v[2 * i + 1] * sn[i];
-                    o[2 * i + 1] = v[2 * i] * sn[i] + v[2 * i + 1] * cs[i];
+            for (int k = 0; k < 4; ++k) {
+                const int h = hb + k * a.hs;
+                if (h < a.H) {
+                    r[k] = xload<T>(x + h * a.xhs, ne);
+                    if (!INTERLEAVED && rot) q[k] = xload<T>(x + h * a.xhs + a.pairs, ne);
                 }
-                xstore<T>(y, ne, o);
-            } else {
-                float w[V], o2[V];
-                xload<T>(x + a.pairs, ne, w);
+            }
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int k = i < NP ? i : 0;
-                    o[i] = v[i] * cs[k] - w[i] * sn[k];
-                    o2[i] = v[i] * sn[k] + w[i] * cs[k];
+            for (int k = 0; k < 4; ++k) {
+                const int h = hb + k * a.hs;
+                if (h >= a.H) break;
+                T* d = y + h * a.yhs;
+                float v[V], o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = (float)r[k][i];
+                if (!rot) {
+                    xstore<T>(d, ne, v);
+                } else if (INTERLEAVED) {
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i) {
+                        o[2 * i] = v[2 * i] * cs[i] - v[2 * i + 1] * sn[i];
+                        o[2 * i + 1] = v[2 * i] * sn[i] + v[2 * i + 1] * cs[i];
+                    }
+                    xstore<T>(d, ne, o);
+                } else {
+                    float o2[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const int j = i < NP ? i : 0;
+                        const float w = (float)q[k][i];
+                        o[i] = v[i] * cs[j] - w * sn[j];
+                        o2[i] = v[i] * sn[j] + w * cs[j];
+                    }
+                    xstore<T>(d, ne, o);
+                    xstore<T>(d + a.pairs, ne, o2);
                 }
-                xstore<T>(y, ne, o);
-                xstore<T>(y + a.pairs, ne, o2);
             }
         }
     }

@@ -594,25 +594,19 @@ class FrameNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, eps):
-        ops._require_cuda(x)
-        x2 = ops.feature_rows(x.detach())
-        needs = any(ctx.needs_input_grad[:3])
-        y, stats = ops.frame_norm_fwd(x2, None if gamma is None else gamma.detach().contiguous(),
-                                      None if beta is None else beta.detach().contiguous(), eps, want_stats=needs)
-        if needs:
-            ctx.save_for_backward(x, gamma, stats)
-            ctx.beta_dtype = None if beta is None else beta.dtype
-        return y.view(x.shape)
+        y, stats = ops.frame_norm_fwd(ops.feature_rows(x), gamma, beta, eps)
+        ctx.save_for_backward(x, gamma, stats)
+        ctx.beta_dtype = None if beta is None else beta.dtype
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, gamma, stats = ctx.saved_tensors
-        dx, dgamma, dbeta = ops.frame_norm_bwd(
-            ops.feature_rows(dy), ops.feature_rows(x), None if gamma is None else gamma.contiguous(), stats,
-            ctx.needs_input_grad[0], gamma.dtype if ctx.needs_input_grad[1] else None,
-            ctx.beta_dtype if ctx.needs_input_grad[2] else None)
-        return None if dx is None else dx.view(x.shape), dgamma, dbeta, None
+        need_x, need_g, need_b, _ = ctx.needs_input_grad
+        dx, dgamma, dbeta = ops.frame_norm_bwd(ops.feature_rows(dy), ops.feature_rows(x), gamma, stats, need_x,
+                                               gamma.dtype if need_g else None, ctx.beta_dtype if need_b else None)
+        return dx if dx is None or x.dim() == 2 else dx.view(x.shape), dgamma, dbeta, None
 
 
 class RotaryFn(torch.autograd.Function):
@@ -620,10 +614,9 @@ class RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, turns, positions, first, interleaved, magnitude):
-        ops._require_cuda(x)
         ctx.meta = (first, interleaved, magnitude)
         ctx.save_for_backward(turns, positions)
-        return ops.rotary(x.detach(), turns, positions, first, interleaved, False, magnitude)
+        return ops.rotary(x, turns, positions, first, interleaved, False, magnitude)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -639,12 +632,9 @@ class AttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, causal, scale):
-        ops._require_cuda(q, k, v)
-        needs = any(ctx.needs_input_grad[:3])
-        o, lse = ops.attn_fwd(q.detach(), k.detach(), v.detach(), lengths, causal, scale, want_lse=needs)
-        if needs:
-            ctx.save_for_backward(q, k, v, o, lse, lengths)
-            ctx.meta = (causal, scale)
+        o, lse = ops.attn_fwd(q, k, v, lengths, causal, scale)
+        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        ctx.meta = (causal, scale)
         return o
 
     @staticmethod

@@ -6,6 +6,7 @@ import math
 import torch
 import torch.nn as nn
 
+from .. import ops
 from ..functional import AttentionFn, LinearFn, RotaryFn
 
 
@@ -24,7 +25,9 @@ def attention(q, k, v, lengths=None, causal=False, scale=None):
     Returns:
         output (B, Tq, H, D), dense
     """
-    return AttentionFn.apply(q, k, v, lengths, bool(causal), scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return AttentionFn.apply(q, k, v, lengths, causal, scale)
+    return ops.attn_fwd(q, k, v, lengths, causal, scale, want_lse=False)[0]
 
 
 def rotate(input, turns, positions=None, offset=0, interleaved=False, magnitude=1.0):
@@ -36,7 +39,9 @@ def rotate(input, turns, positions=None, offset=0, interleaved=False, magnitude=
         positions: whole numbers (T,) or (B, T) on the input's device; None: offset, offset + 1, ...
         interleaved: pairs (2 i, 2 i + 1) instead of (i, i + len(turns))
     """
-    return RotaryFn.apply(input, turns, positions, int(offset), bool(interleaved), float(magnitude))
+    if torch.is_grad_enabled() and input.requires_grad:
+        return RotaryFn.apply(input, turns, positions, offset, interleaved, magnitude)
+    return ops.rotary(input, turns, positions, offset, interleaved, False, magnitude)
 
 
 def rotary_turns(rotary_dim, base=10000.0, scaling=None):

@@ -4,6 +4,7 @@ reference does not have."""
 import torch
 import torch.nn as nn
 
+from .. import ops
 from ..functional import FrameNormFn, LayerNormFn
 
 EPS = 1e-12
@@ -70,13 +71,17 @@ def frame_layer_norm(input, weight=None, bias=None, eps=EPS):
 
     Args:
         input (..., C), float32 or bfloat16, C up to 16384
-        weight, bias (C,) in float32 or the input's type, or None
+        weight, bias (C,) in float32 or the input's type (contiguous), or None
     Returns:
         output: same shape and type as the input (dense)
     """
     if input.dim() < 1 or input.size(-1) < 1:
         raise ValueError("frame_layer_norm needs at least one feature, got {}".format(tuple(input.shape)))
-    return FrameNormFn.apply(input, weight, bias, eps)
+    if torch.is_grad_enabled() and (input.requires_grad or weight is not None and weight.requires_grad or
+                                    bias is not None and bias.requires_grad):
+        return FrameNormFn.apply(input, weight, bias, eps)
+    y, _ = ops.frame_norm_fwd(ops.feature_rows(input), weight, bias, eps, want_stats=False)
+    return y if input.dim() == 2 else y.view(input.shape)
 
 
 class FrameLayerNorm(nn.Module):

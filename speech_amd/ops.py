@@ -7,7 +7,9 @@ stride whose row and batch strides are multiples of 4 floats ("act" layout,
 see new_act); anything else is copied into that layout first.
 """
 import ctypes as C
+import functools
 import os
+import struct
 
 import torch
 
@@ -361,6 +363,7 @@ def rows_wgrad(dy, x, dW=None, dbias=None, sign=1.0, arith=None):
 
 # ------------------------------------------------------------------------------------------------ axis shuffles
 # ------------------------------------------------------------------------------------------------ frame norm, rotary positions, attention
+# (written for their host time: single tokens and short batches cost less on the GPU than in these functions)
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
 FRAME_NORM_MAX_FEATURES = 16384
 ATTENTION_MAX_HEAD = 128
@@ -380,40 +383,58 @@ def _same_place(what, first, *rest):
             raise _lib.CtnError("{}: tensors on {} and {}".format(what, first.device, t.device))
 
 
-def _enqueue(name, t, fn, *args):
-    """fn(*args, stream) on the current stream of t's device, which need not be the current device."""
-    if t.device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
-        return
-    with torch.cuda.device(t.device):
-        _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+def _enqueue(name, device, fn, *args):
+    """fn(*args, stream) on the current stream of a device (its index), which need not be the current device."""
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def feature_rows(x):
     """(..., C) as (rows, C) with unit feature stride: a view where the strides allow it."""
-    x2 = x.reshape(-1, x.shape[-1])
-    return x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _frame_norm_ws(R, Cc, code):
+    return _lib.load().ctn_frame_norm_bwd_ws_floats(R, Cc, code)
+
+
+def _frame_norm_param_type(x2, gamma, beta):
+    """CTN_TYPE_* of the parameters, which are checked."""
+    code = _type(x2, "frame_norm")
+    if gamma is None and beta is None:
+        return code, code
+    _same_place("frame_norm", x2, gamma, beta)
+    dt = None
+    for w in (gamma, beta):
+        if w is None:
+            continue
+        if w.numel() != x2.shape[1] or not w.is_contiguous():
+            raise _lib.CtnError("frame_norm: parameters of {} contiguous elements, got {}".format(x2.shape[1], tuple(w.shape)))
+        if w.dtype != torch.float32 and w.dtype != x2.dtype or dt is not None and w.dtype != dt:
+            raise _lib.CtnError("frame_norm: parameters in float32 or the input's type, both alike")
+        dt = w.dtype
+    return code, _TYPES[dt]
 
 
 def frame_norm_fwd(x2, gamma, beta, eps, want_stats=True):
     """x2 (R, C) rows -> y (R, C), stats (3, R) for frame_norm_bwd (None unless wanted); see ctn_frame_norm_fwd."""
     lib = _lib.load()
-    _same_place("frame_norm", x2, gamma, beta)
+    code, wcode = _frame_norm_param_type(x2, gamma, beta)
+    if not x2.is_cuda:
+        _require_cuda(x2)
     R, Cc = x2.shape
-    code = _type(x2, "frame_norm")
-    wcode = code
-    for w in (gamma, beta):
-        if w is None:
-            continue
-        if w.numel() != Cc or not w.is_contiguous():
-            raise _lib.CtnError("frame_norm: parameters of {} contiguous elements, got {}".format(Cc, tuple(w.shape)))
-        wcode = _type(w, "frame_norm")
-    if (gamma is not None and beta is not None and gamma.dtype != beta.dtype) or wcode not in (_lib.TYPE_F32, code):
-        raise _lib.CtnError("frame_norm: parameters in float32 or the input's type, both alike")
-    y = torch.empty((R, Cc), device=x2.device, dtype=x2.dtype)
-    stats = torch.empty((3, R), device=x2.device, dtype=torch.float32) if want_stats else None
-    _enqueue("ctn_frame_norm_fwd", x2, lib.ctn_frame_norm_fwd, _ptr(x2), _ld(x2), R, Cc, code, _ptr(gamma), _ptr(beta), wcode,
-             float(eps), _ptr(y), Cc, _ptr(stats))
+    y = x2.new_empty((R, Cc))
+    stats = x2.new_empty((3, R), dtype=torch.float32) if want_stats else None
+    _enqueue("ctn_frame_norm_fwd", x2.get_device(), lib.ctn_frame_norm_fwd, x2.data_ptr(), x2.stride(0) if R > 1 else Cc, R, Cc,
+             code, _ptr(gamma), _ptr(beta), wcode, eps, y.data_ptr(), Cc, _ptr(stats))
     return y, stats
 
 
@@ -421,24 +442,19 @@ def frame_norm_bwd(dy2, x2, gamma, stats, want_dx=True, want_dgamma=None, want_d
     """-> dx (R, C), dgamma (C,), dbeta (C,), each None unless wanted (want_dgamma / want_dbeta: the parameter's dtype);
     see ctn_frame_norm_bwd."""
     lib = _lib.load()
-    _same_place("frame_norm", x2, dy2, gamma, stats)
     R, Cc = x2.shape
     code = _type(x2, "frame_norm")
-    assert dy2.shape == x2.shape and dy2.dtype == x2.dtype
-    dev = x2.device
+    assert dy2.shape == x2.shape and dy2.dtype == x2.dtype and dy2.device == x2.device
     wdtype = want_dgamma or want_dbeta or (torch.float32 if gamma is None else gamma.dtype)
-    dx = torch.empty((R, Cc), device=dev, dtype=x2.dtype) if want_dx else None
-    dgamma = torch.empty((Cc,), device=dev, dtype=wdtype) if want_dgamma else None
-    dbeta = torch.empty((Cc,), device=dev, dtype=wdtype) if want_dbeta else None
-    need = lib.ctn_frame_norm_bwd_ws_floats(R, Cc, code) if want_dgamma or want_dbeta else 0
-    ws = torch.empty((need,), device=dev, dtype=torch.float32) if need else None
-    _enqueue("ctn_frame_norm_bwd", x2, lib.ctn_frame_norm_bwd, _ptr(dy2), _ld(dy2), _ptr(x2), _ld(x2), R, Cc, code,
-             _ptr(gamma), _TYPES[wdtype], _ptr(stats), _ptr(dx), Cc, _ptr(dgamma), _ptr(dbeta), _ptr(ws), need)
+    dx = x2.new_empty((R, Cc)) if want_dx else None
+    dgamma = x2.new_empty((Cc,), dtype=wdtype) if want_dgamma else None
+    dbeta = x2.new_empty((Cc,), dtype=wdtype) if want_dbeta else None
+    need = _frame_norm_ws(R, Cc, code) if want_dgamma or want_dbeta else 0
+    ws = x2.new_empty((need,), dtype=torch.float32) if need else None
+    _enqueue("ctn_frame_norm_bwd", x2.get_device(), lib.ctn_frame_norm_bwd, dy2.data_ptr(), dy2.stride(0) if R > 1 else Cc,
+             x2.data_ptr(), x2.stride(0) if R > 1 else Cc, R, Cc, code, _ptr(gamma), _TYPES[wdtype], stats.data_ptr(), _ptr(dx), Cc,
+             _ptr(dgamma), _ptr(dbeta), _ptr(ws), need)
     return dx, dgamma, dbeta
-
-
-def _unit_last(x):
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
 def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, magnitude=1.0):
@@ -449,115 +465,137 @@ def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, 
     code = _type(x, "rotary")
     if x.dim() != 4:
         raise _lib.CtnError("rotary: a (batch, tokens, heads, features) tensor, got {} dimensions".format(x.dim()))
-    B, T, H, D = x.shape
-    if turns.dtype != torch.float64 or turns.dim() != 1 or 2 * turns.numel() > D:
+    B, T, H, D = shape = x.shape
+    pairs = turns.numel()
+    if turns.dtype != torch.float64 or turns.dim() != 1 or 2 * pairs > D:
         raise _lib.CtnError("rotary: turns in float64, at most {} of them for {} features".format(D // 2, D))
-    turns = turns.contiguous()
-    pbs = 0
+    if not turns.is_contiguous():
+        turns = turns.contiguous()
+    pbs, pptr = 0, None
     if positions is not None:
-        if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) not in ((T,), (B, T)):
+        ps = tuple(positions.shape)
+        if positions.dtype not in (torch.int64, torch.int32) or (ps != (T,) and ps != (B, T)):
             raise _lib.CtnError("rotary: whole positions of shape ({},) or ({}, {}), got {} {}".format(
-                T, B, T, positions.dtype, tuple(positions.shape)))
-        positions = positions.to(torch.int64).contiguous()
-        pbs = T if positions.dim() == 2 else 0
-    x = _unit_last(x)
-    y = torch.empty((B, T, H, D), device=x.device, dtype=x.dtype)
-    _enqueue("ctn_rotary", x, lib.ctn_rotary, _ptr(x), x.stride(0), x.stride(1), x.stride(2), B, T, H, D, code,
-             _ptr(positions), pbs, int(first), _ptr(turns), 2 * turns.numel(), 1 if interleaved else 0, 1 if inverse else 0,
-             float(magnitude), _ptr(y), y.stride(0), y.stride(1), y.stride(2))
+                T, B, T, positions.dtype, ps))
+        if positions.dtype != torch.int64 or not positions.is_contiguous():
+            positions = positions.to(torch.int64).contiguous()
+        pbs, pptr = (T if len(ps) == 2 else 0), positions.data_ptr()
+    xb, xt, xh, xd = x.stride()
+    if xd != 1 and D != 1:
+        x = x.contiguous()
+        xb, xt, xh, xd = x.stride()
+    y = x.new_empty(shape)
+    _enqueue("ctn_rotary", x.get_device(), lib.ctn_rotary, x.data_ptr(), xb, xt, xh, B, T, H, D, code, pptr, pbs, first,
+             turns.data_ptr(), 2 * pairs, 1 if interleaved else 0, 1 if inverse else 0, magnitude, y.data_ptr(), T * H * D, H * D, D)
     return y
 
 
-def _attn_operand(x):
-    """x with unit feature stride, 16-byte aligned, all strides whole 16 bytes: itself or a dense copy."""
-    per = 16 // x.element_size()
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(x.stride(i) % per == 0 or x.shape[i] == 1 for i in range(3)):
-        return x
-    return x.contiguous()
+def _attn_operand(x, shape):
+    """x with unit feature stride, 16-byte aligned, all strides whole 16 bytes (itself or a dense copy), and its strides."""
+    b, t, h, d = x.stride()
+    m = 3 if x.dtype == torch.float32 else 7
+    if d != 1 or x.data_ptr() & 15 or (b | t | h) & m:
+        if shape[0] == 1:
+            b = 0
+        if shape[1] == 1:
+            t = 0
+        if shape[2] == 1:
+            h = 0
+        if d != 1 or x.data_ptr() & 15 or (b | t | h) & m:
+            x = x.contiguous()
+            t, h = shape[2] * shape[3], shape[3]
+            b = shape[1] * t
+    return x, b, t, h
 
 
-def _attn_strides(x):
-    return tuple(0 if x.shape[i] == 1 else x.stride(i) for i in range(3))
-
-
-def _attn_args(q, k, v, o, lse, lengths, causal, scale):
-    B, Tq, H, D = q.shape
-    a = _lib.AttnArgs()
-    a.batch, a.Tq, a.Tk, a.H, a.Hk, a.D = B, Tq, k.shape[1], H, k.shape[2], D
-    a.type, a.causal, a.scale = _TYPES[q.dtype], 1 if causal else 0, scale
-    a.lengths = _ptr(lengths)
-    a.q, a.k, a.v, a.o, a.lse = _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse)
-    a.q_b, a.q_t, a.q_h = _attn_strides(q)
-    a.k_b, a.k_t, a.k_h = _attn_strides(k)
-    a.v_b, a.v_t, a.v_h = _attn_strides(v)
-    a.o_b, a.o_t, a.o_h = _attn_strides(o)
-    return a
+# the fields of ctn_attn_args in their order
+_ATTN_PACK = struct.Struct("8if i" + "Q" + "Qqqq" * 4 + "Q" + "Qqqq" * 4 + "Qq").pack
+_ATTN_NONE = (0, 0, 0, 0)
 
 
 def check_attention(q, k, v, lengths):
     """Raises CtnError unless attn_fwd takes these tensors."""
     _same_place("attention", q, k, v, lengths)
     code = _type(q, "attention")
-    if any(t.dim() != 4 for t in (q, k, v)) or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[3] != ks[3]:
         raise _lib.CtnError("attention: q (B, Tq, H, D), k and v (B, Tk, Hk, D), got {}, {}, {}".format(
-            tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if _TYPES.get(k.dtype) != code or _TYPES.get(v.dtype) != code:
+            tuple(qs), tuple(ks), tuple(v.shape)))
+    if k.dtype != q.dtype or v.dtype != q.dtype:
         raise _lib.CtnError("attention: q, k and v of one type, got {}, {}, {}".format(q.dtype, k.dtype, v.dtype))
-    H, Hk, D = q.shape[2], k.shape[2], q.shape[3]
+    H, Hk, D = qs[2], ks[2], qs[3]
     if Hk < 1 or H < 1 or H % Hk:
         raise _lib.CtnError("attention: {} query heads for {} key heads (a multiple)".format(H, Hk))
     if D % 8 or not 8 <= D <= ATTENTION_MAX_HEAD:
         raise _lib.CtnError("attention: {} features per head (multiples of 8 up to {})".format(D, ATTENTION_MAX_HEAD))
-    if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (q.shape[0],)):
+    if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (qs[0],)):
         raise _lib.CtnError("attention: whole lengths of shape ({},), got {} {}".format(
-            q.shape[0], lengths.dtype, tuple(lengths.shape)))
+            qs[0], lengths.dtype, tuple(lengths.shape)))
+    return code
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_ws(B, Tq, Tk, H, Hk, D, code, backward):
+    """Workspace floats of a call of these sizes."""
+    a = _lib.AttnArgs(batch=B, Tq=Tq, Tk=Tk, H=H, Hk=Hk, D=D, type=code, scale=1.0, q=16, k=16, v=16, o=16)
+    lib = _lib.load()
+    return max(0, (lib.ctn_attn_bwd_ws_floats if backward else lib.ctn_attn_fwd_ws_floats)(C.byref(a)))
+
+
+def _attn_lengths(lengths, Tk):
+    if lengths is None:
+        return None
+    if lengths.dtype != torch.int32:
+        lengths = lengths.clamp(0, Tk).to(torch.int32)
+    return lengths.contiguous()
 
 
 def attn_fwd(q, k, v, lengths=None, causal=False, scale=None, want_lse=True):
     """q (B, Tq, H, D), k, v (B, Tk, Hk, D) -> o dense like q, lse (B, H, Tq) fp32 (None unless wanted); see ctn_attn_fwd."""
     lib = _lib.load()
-    check_attention(q, k, v, lengths)
-    B, Tq, H, D = q.shape
-    scale = D ** -0.5 if scale is None else float(scale)
-    q, k, v = _attn_operand(q), _attn_operand(k), _attn_operand(v)
-    if lengths is not None:
-        lengths = lengths.clamp(0, k.shape[1]).to(torch.int32) if lengths.dtype == torch.int64 else lengths
-        lengths = lengths.contiguous()
-    o = torch.empty((B, Tq, H, D), device=q.device, dtype=q.dtype)
-    lse = torch.empty((B, H, Tq), device=q.device, dtype=torch.float32) if want_lse else None
-    a = _attn_args(q, k, v, o, lse, lengths, causal, scale)
-    need = lib.ctn_attn_fwd_ws_floats(C.byref(a))
-    ws = torch.empty((need,), device=q.device, dtype=torch.float32) if need > 0 else None
-    a.ws, a.ws_floats = _ptr(ws), max(need, 0)
-    _enqueue("ctn_attn_fwd", q, lib.ctn_attn_fwd, C.byref(a))
+    code = check_attention(q, k, v, lengths)
+    B, Tq, H, D = qs = q.shape
+    _, Tk, Hk, _ = ks = k.shape
+    q, qb, qt, qh = _attn_operand(q, qs)
+    k, kb, kt, kh = _attn_operand(k, ks)
+    v, vb, vt, vh = _attn_operand(v, ks)
+    lengths = _attn_lengths(lengths, Tk)
+    o = q.new_empty(qs)
+    lse = q.new_empty((B, H, Tq), dtype=torch.float32) if want_lse else None
+    need = _attn_ws(B, Tq, Tk, H, Hk, D, code, False)
+    ws = q.new_empty((need,), dtype=torch.float32) if need else None
+    args = _lib.AttnArgs.from_buffer_copy(_ATTN_PACK(
+        B, Tq, Tk, H, Hk, D, code, 1 if causal else 0, D ** -0.5 if scale is None else scale, 0, _ptr(lengths) or 0,
+        q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, o.data_ptr(), Tq * H * D, H * D, D,
+        _ptr(lse) or 0, *_ATTN_NONE, *_ATTN_NONE, *_ATTN_NONE, *_ATTN_NONE, _ptr(ws) or 0, need))
+    _enqueue("ctn_attn_fwd", q.get_device(), lib.ctn_attn_fwd, args)
     return o, lse
 
 
 def attn_bwd(do, q, k, v, o, lse, lengths=None, causal=False, scale=None, want=(True, True, True)):
     """-> dq, dk, dv (dense, each None unless wanted) from the gradient of o and what attn_fwd returned; see ctn_attn_bwd."""
     lib = _lib.load()
-    check_attention(q, k, v, lengths)
-    _same_place("attention", q, do, o, lse)
-    assert do.shape == q.shape and do.dtype == q.dtype
-    B, Tq, H, D = q.shape
-    scale = D ** -0.5 if scale is None else float(scale)
-    q, k, v, do = _attn_operand(q), _attn_operand(k), _attn_operand(v), _attn_operand(do)
-    if lengths is not None:
-        lengths = lengths.clamp(0, k.shape[1]).to(torch.int32) if lengths.dtype == torch.int64 else lengths
-        lengths = lengths.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if w else None for t, w in zip((q, k, v), want))
-    a = _attn_args(q, k, v, o, lse, lengths, causal, scale)
-    a.d_o, (a.do_b, a.do_t, a.do_h) = _ptr(do), _attn_strides(do)
-    if dq is not None:
-        a.dq, (a.dq_b, a.dq_t, a.dq_h) = _ptr(dq), _attn_strides(dq)
-    if dk is not None:
-        a.dk, (a.dk_b, a.dk_t, a.dk_h) = _ptr(dk), _attn_strides(dk)
-    if dv is not None:
-        a.dv, (a.dv_b, a.dv_t, a.dv_h) = _ptr(dv), _attn_strides(dv)
-    need = lib.ctn_attn_bwd_ws_floats(C.byref(a))
-    ws = torch.empty((need,), device=q.device, dtype=torch.float32) if need > 0 else None
-    a.ws, a.ws_floats = _ptr(ws), max(need, 0)
-    _enqueue("ctn_attn_bwd", q, lib.ctn_attn_bwd, C.byref(a))
+    code = check_attention(q, k, v, lengths)
+    B, Tq, H, D = qs = q.shape
+    _, Tk, Hk, _ = ks = k.shape
+    assert do.shape == qs and do.dtype == q.dtype and do.device == q.device and o.is_contiguous() and o.shape == qs
+    q, qb, qt, qh = _attn_operand(q, qs)
+    k, kb, kt, kh = _attn_operand(k, ks)
+    v, vb, vt, vh = _attn_operand(v, ks)
+    do, gb, gt, gh = _attn_operand(do, qs)
+    lengths = _attn_lengths(lengths, Tk)
+    dq = q.new_empty(qs) if want[0] else None
+    dk = q.new_empty(ks) if want[1] else None
+    dv = q.new_empty(ks) if want[2] else None
+    need = _attn_ws(B, Tq, Tk, H, Hk, D, code, True)
+    ws = q.new_empty((need,), dtype=torch.float32) if need else None
+    dense_k = (Tk * Hk * D, Hk * D, D)
+    args = _lib.AttnArgs.from_buffer_copy(_ATTN_PACK(
+        B, Tq, Tk, H, Hk, D, code, 1 if causal else 0, D ** -0.5 if scale is None else scale, 0, _ptr(lengths) or 0,
+        q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, o.data_ptr(), Tq * H * D, H * D, D,
+        lse.data_ptr(), do.data_ptr(), gb, gt, gh, _ptr(dq) or 0, Tq * H * D, H * D, D, _ptr(dk) or 0, *dense_k,
+        _ptr(dv) or 0, *dense_k, _ptr(ws) or 0, need))
+    _enqueue("ctn_attn_bwd", q.get_device(), lib.ctn_attn_bwd, args)
     return dq, dk, dv
 
 
