@@ -100,29 +100,54 @@ template <int DT> __device__ __forceinline__ int img(const int r, const int ch) 
     return 2 * DT * r + 16 * (ch ^ key);
 }
 
-// Tile of ROWS x DT elements staged by NT threads: thread's chunk i is chunk (tid + NT i) of the tile, row by row
+// Tile of ROWS x DT elements staged by NT threads: thread's chunk i is chunk (tid + NT i) of the tile, row by row.  The
+// loads are buffer loads with one 32-bit offset per chunk, computed once: a tile's descriptor starts at its first row and
+// ends behind its last valid one, so rows beyond it (and the features from D on, whose offset lies behind any
+// descriptor) come back as zeros and touch no memory.  That wants rows that do not overlap, and a row stride of less than
+// MAX_PITCH bytes.
+constexpr int64_t MAX_PITCH = 1 << 24;
+
 template <typename T, int DT, int ROWS, int NT> struct Tile {
-    static constexpr int CPR = DT / 8, N = ROWS * CPR / NT, PLANE = ROWS * DT * 2;
+    static constexpr int CPR = DT / 8, N = (ROWS * CPR + NT - 1) / NT, PLANE = ROWS * DT * 2, ES = sizeof(T);
     static constexpr int BYTES = Planes<T>::N * PLANE;
-    static_assert(ROWS * CPR % NT == 0, "whole chunks per thread");
-    Chunk<T> c[N];
-    // rows 0 .. nvalid - 1 at base + row * stride, D elements each; everything else zero
-    __device__ __forceinline__ void load(const T* __restrict__ base, const int64_t stride, const int nvalid, const int D) {
+    static constexpr bool WHOLE = ROWS * CPR % NT == 0;
+    static constexpr int QUADS = ES == 4 ? 2 : 1;                // 16-byte loads per chunk
+    u32x4 c[N][QUADS];
+    int off[N];
+    int pitch;                                                   // bytes
+    __device__ __forceinline__ void init(const int64_t stride, const int D) {
+        pitch = (int)stride * ES;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int q = threadIdx.x + NT * i, r = q / CPR, d = (q % CPR) * 8;
-            if (r < nvalid && d < D) c[i].load(base + r * stride + d);
-            else c[i].zero();
+            off[i] = (WHOLE || r < ROWS) && d < D ? r * pitch + d * ES : 0x7fffff00;
         }
+    }
+    // rows 0 .. nvalid - 1 at base, D elements each; everything else zero
+    __device__ __forceinline__ void load(const T* base, const int nvalid, const int D) {
+        const int rows = nvalid < ROWS ? nvalid : ROWS;
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows > 0 ? (rows - 1) * pitch + D * ES : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int h = 0; h < QUADS; ++h) c[i][h] = __builtin_amdgcn_raw_buffer_load_b128(r, off[i] + 16 * h, 0, 0);
     }
     __device__ __forceinline__ void store(unsigned char* lds) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int q = threadIdx.x + NT * i, r = q / CPR, ch = q % CPR;
             Frag<Planes<T>::N> f;
-            c[i].frag(f);
+            if constexpr (ES == 2) {
+                f.p[0] = __builtin_bit_cast(bf16x8, c[i][0]);
+            } else {
+                float x[8];
 #pragma unroll
-            for (int p = 0; p < Planes<T>::N; ++p) *reinterpret_cast<bf16x8*>(lds + p * PLANE + img<DT>(r, ch)) = f.p[p];
+                for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(c[i][QUADS == 2 ? j >> 2 : 0][j & 3]);
+                make_frag(x, f);
+            }
+            if (WHOLE || r < ROWS)
+#pragma unroll
+                for (int p = 0; p < Planes<T>::N; ++p) *reinterpret_cast<bf16x8*>(lds + p * PLANE + img<DT>(r, ch)) = f.p[p];
         }
     }
 };
@@ -183,9 +208,12 @@ __device__ __forceinline__ unsigned die_order(const unsigned id, const unsigned 
     return x < r ? x * (q + 1) + i : r * (q + 1) + (x - r) * q + i;
 }
 
-static inline bool strides_ok(const void* p, int64_t b, int64_t t, int64_t h, int es) {
+// 16-byte aligned, strides of whole 16 bytes; rows (of D elements, T of them) that do not overlap and lie less than
+// MAX_PITCH bytes apart
+static inline bool strides_ok(const void* p, int64_t b, int64_t t, int64_t h, int es, int D, int T) {
     const int64_t m = 16 / es;
-    return ctn_aligned16(p) && b % m == 0 && t % m == 0 && h % m == 0 && b >= 0 && t >= 0 && h >= 0;
+    return ctn_aligned16(p) && b % m == 0 && t % m == 0 && h % m == 0 && b >= 0 && h >= 0 &&
+           (T <= 1 || (t >= D && t * es < MAX_PITCH));
 }
 
 }  // namespace attn

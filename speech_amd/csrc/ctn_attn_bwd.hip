@@ -55,16 +55,21 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const bwd_params f) {
 
     const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h;
     const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h;
+    const int64_t kstep = KT * a.k_t, vstep = KT * a.v_t;
+    int left = kend;
     tile_t tk, tv;
-    auto fetch = [&](const int t) {
-        tk.load(kp + (int64_t)t * KT * a.k_t, a.k_t, kend - t * KT, a.D);
-        tv.load(vp + (int64_t)t * KT * a.v_t, a.v_t, kend - t * KT, a.D);
+    tk.init(a.k_t, a.D);
+    tv.init(a.v_t, a.D);
+    auto fetch = [&]() {                                         // the next tile
+        tk.load(kp, left, a.D);
+        tv.load(vp, left, a.D);
+        kp += kstep, vp += vstep, left -= KT;
     };
     auto stage = [&](const int buf) {
         tk.store(lds + buf * BUF);
         tv.store(lds + buf * BUF + tile_t::BYTES);
     };
-    if (t1 > 0) fetch(0);
+    if (t1 > 0) fetch();
 
     Frag<NP> q[KS], g[KS];
     float delta = 0.f;
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const bwd_params f) {
     for (int t = 0; t < t1; ++t) {
         const unsigned char* K = lds + (t & 1) * BUF;
         const unsigned char* V = K + tile_t::BYTES;
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) fetch();
 #pragma unroll
         for (int r0 = 0; r0 < KT; r0 += 32) {
             const int k0 = t * KT + r0;
@@ -195,12 +200,14 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
     }
 
     tile_t tq, tg;
+    tq.init(a.q_t, a.D);
+    tg.init(a.do_t, a.D);
     constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
     float stat[NS];
     auto fetch = [&](const int i) {
         const int head = hk * f.G + i / nq, q0 = (t0 + i % nq) * QT;
-        tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.q_t, a.Tq - q0, a.D);
-        tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.do_t, a.Tq - q0, a.D);
+        tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.Tq - q0, a.D);
+        tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.Tq - q0, a.D);
 #pragma unroll
         for (int x = 0; x < NS; ++x) {
             const int j = threadIdx.x + NT * x, r = q0 + j % QT;
@@ -339,11 +346,11 @@ int ctn_attn_bwd(const ctn_attn_args* a, void* stream) {
     if (a->batch == 0) return CTN_OK;
     const int es = a->type == CTN_TYPE_F32 ? 4 : 2;
     const int64_t nrow = (int64_t)a->batch * a->H * a->Tq;
-    CTN_REQUIRE(a->Tq == 0 || (a->d_o && a->lse && strides_ok(a->d_o, a->do_b, a->do_t, a->do_h, es)),
-                "ctn_attn_bwd: d_o (16-byte aligned, strides of whole 16 bytes) and lse are needed");
-    CTN_REQUIRE((!a->dq || strides_ok(a->dq, a->dq_b, a->dq_t, a->dq_h, es)) &&
-                    (!a->dk || strides_ok(a->dk, a->dk_b, a->dk_t, a->dk_h, es)) &&
-                    (!a->dv || strides_ok(a->dv, a->dv_b, a->dv_t, a->dv_h, es)),
+    CTN_REQUIRE(a->Tq == 0 || (a->d_o && a->lse && strides_ok(a->d_o, a->do_b, a->do_t, a->do_h, es, a->D, a->Tq)),
+                "ctn_attn_bwd: d_o (as q, k, v: aligned, rows apart) and lse are needed");
+    CTN_REQUIRE((!a->dq || strides_ok(a->dq, a->dq_b, a->dq_t, a->dq_h, es, a->D, a->Tq)) &&
+                    (!a->dk || strides_ok(a->dk, a->dk_b, a->dk_t, a->dk_h, es, a->D, a->Tk)) &&
+                    (!a->dv || strides_ok(a->dv, a->dv_b, a->dv_t, a->dv_h, es, a->D, a->Tk)),
                 "ctn_attn_bwd: dq, dk, dv must be 16-byte aligned with strides of whole 16 bytes");
     CTN_REQUIRE(nrow == 0 || (a->ws && a->ws_floats >= nrow), "ctn_attn_bwd: workspace of %lld floats, %lld needed",
                 (long long)a->ws_floats, (long long)nrow);

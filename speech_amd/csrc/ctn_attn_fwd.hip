@@ -21,9 +21,15 @@ struct fwd_params {
     float* po; float* pl;                 // split: partial outputs [nsplit][B H Tq][D] and log2-sums [nsplit][B H Tq]
 };
 
-template <typename T, int DT, int NW, int KT>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(const fwd_params f) {
-    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, NK = KT / 32, ND = DT / 32;
+#ifndef WPE
+#define WPE 2
+#endif
+#ifndef PRIO
+#define PRIO 0
+#endif
+template <typename T, int DT, int NW, int QW, int KT>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) void attn_fwd_kernel(const fwd_params f) {
+    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, NK = KT / 32, ND = DT / 32, ROWS = 32 * QW;
     typedef Tile<T, DT, KT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES;                       // a buffer: K planes, V planes
     __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
@@ -39,119 +45,154 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(const fwd_params f) {
     id /= f.nqt;
     const int hh = id % f.heads, b = id / f.heads;
 
-    const int w0 = qt * 32 * NW + wave * 32;                     // the wave's first row
-    const int n = w0 + (lane & 31);
-    const bool live = n < f.rows;
-    const int g = f.packed ? n / a.Tq : 0, tq = f.packed ? n - g * a.Tq : n;
-    const int hk = f.packed ? hh : hh / f.G, head = f.packed ? hh * f.G + g : hh;
-
+    const int w0 = (qt * NW + wave) * ROWS;                      // the wave's first row
+    const int hk = f.packed ? hh : hh / f.G;
     int len = a.Tk;
     if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
-    const int vis = !live ? 0 : a.causal ? min(len, tq + off + 1) : len;         // keys 0 .. vis - 1 are visible
+    int vis[QW], tq[QW], head[QW];                               // keys 0 .. vis - 1 are visible to the lane's rows
+    bool live[QW];
+#pragma unroll
+    for (int w = 0; w < QW; ++w) {
+        const int n = w0 + 32 * w + (lane & 31);
+        live[w] = n < f.rows;
+        const int g = f.packed ? n / a.Tq : 0;
+        tq[w] = f.packed ? n - g * a.Tq : n;
+        head[w] = f.packed ? hh * f.G + g : hh;
+        vis[w] = !live[w] ? 0 : a.causal ? min(len, tq[w] + off + 1) : len;
+    }
     // block: keys below kend are read; wave: tiles below wfull need no mask, tiles from wend on hold nothing for it
     int kend = len, wfull = len, wend = len;
     if (a.causal) {
-        const int last = f.packed ? a.Tq - 1 : min(f.rows, (qt + 1) * 32 * NW) - 1;
+        const int last = f.packed ? a.Tq - 1 : min(f.rows, (qt + 1) * ROWS * NW) - 1;
         kend = min(len, last + off + 1);
         wfull = min(len, (f.packed ? 0 : w0) + off + 1);
-        wend = min(len, (f.packed ? a.Tq : min(f.rows, w0 + 32)) + off);
+        wend = min(len, (f.packed ? a.Tq : min(f.rows, w0 + ROWS)) + off);
     }
     if (w0 >= f.rows) wend = 0;
     const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
     const int t0 = (int)((int64_t)ntile * sp / f.nsplit), t1 = (int)((int64_t)ntile * (sp + 1) / f.nsplit);
 
-    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h;
-    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h;
+    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h + (int64_t)t0 * KT * a.k_t;
+    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h + (int64_t)t0 * KT * a.v_t;
+    const int64_t kstep = KT * a.k_t, vstep = KT * a.v_t;
+    int left = kend - t0 * KT;
     tile_t tk, tv;
-    auto fetch = [&](const int t) {
-        tk.load(kp + (int64_t)t * KT * a.k_t, a.k_t, kend - t * KT, a.D);
-        tv.load(vp + (int64_t)t * KT * a.v_t, a.v_t, kend - t * KT, a.D);
+    tk.init(a.k_t, a.D);
+    tv.init(a.v_t, a.D);
+    auto fetch = [&]() {                                         // the next tile
+        tk.load(kp, left, a.D);
+        tv.load(vp, left, a.D);
+        kp += kstep, vp += vstep, left -= KT;
     };
     auto stage = [&](const int buf) {
         tk.store(lds + buf * BUF);
         tv.store(lds + buf * BUF + tile_t::BYTES);
     };
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) fetch();
 
-    Frag<NP> q[KS];
-    {
-        const T* qp = (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
+    Frag<NP> q[QW][KS];
+#pragma unroll
+    for (int w = 0; w < QW; ++w) {
+        const T* qp = (const T*)a.q + b * a.q_b + tq[w] * a.q_t + head[w] * a.q_h;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             Chunk<T> c;
             const int d = 16 * s + 8 * half;
-            if (live && d < a.D) c.load(qp + d);
+            if (live[w] && d < a.D) c.load(qp + d);
             else c.zero();
-            c.frag(q[s]);
+            c.frag(q[w][s]);
         }
     }
-    f32x16 o[ND];
+    f32x16 o[QW][ND];
+    float m[QW], l[QW];
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int w = 0; w < QW; ++w) {
+        m[w] = -INFINITY, l[w] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[w][d][e] = 0.f;
+    }
 
     if (t0 < t1) stage(0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const unsigned char* K = lds + ((t - t0) & 1) * BUF;
         const unsigned char* V = K + tile_t::BYTES;
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) fetch();
         if (t * KT < wend) {
-            f32x16 s[NK];
+            f32x16 s[QW][NK];
 #pragma unroll
-            for (int j = 0; j < NK; ++j)
+            for (int w = 0; w < QW; ++w)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[w][j][e] = 0.f;
+            if (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < KS; ++i)
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
                     Frag<NP> k;
                     frag_rows<NP, DT, KT>(K, 32 * j, i, k);
-                    mma(s[j], k, q[i]);
+#pragma unroll
+                    for (int w = 0; w < QW; ++w) mma(s[w][j], k, q[w][i]);
                 }
+            if (PRIO) __builtin_amdgcn_s_setprio(0);
             if ((t + 1) * KT > wfull) {
+#pragma unroll
+                for (int w = 0; w < QW; ++w) {
+                    const int lim = vis[w] - t * KT - 4 * half;
+#pragma unroll
+                    for (int j = 0; j < NK; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[w][j][e] = 32 * j + (e & 3) + 8 * (e >> 2) < lim ? s[w][j][e] : -INFINITY;
+                }
+            }
+            float base[QW], alpha[QW];
+            bool moved = false;
+#pragma unroll
+            for (int w = 0; w < QW; ++w) {
+                float mx = s[w][0][0];
 #pragma unroll
                 for (int j = 0; j < NK; ++j)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[j][e] = t * KT + 32 * j + acc_row(e) < vis ? s[j][e] : -INFINITY;
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[w][j][e]);
+                const float mn = fmaxf(m[w], half_max(mx));
+                base[w] = mn == -INFINITY ? 0.f : mn * f.sl2;    // rows that see nothing yet stay at zero
+                alpha[w] = __builtin_amdgcn_exp2f(m[w] * f.sl2 - base[w]);
+                moved |= mn != m[w];
+                m[w] = mn;
+                l[w] *= alpha[w];
             }
-            float mx = s[0][0];
+            if (__any(moved)) {
 #pragma unroll
-            for (int j = 0; j < NK; ++j)
+                for (int w = 0; w < QW; ++w)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[j][e]);
-            const float mn = fmaxf(m, half_max(mx));
-            const float base = mn == -INFINITY ? 0.f : mn * f.sl2;           // rows that see nothing yet stay at zero
-            const float alpha = __builtin_amdgcn_exp2f(m == -INFINITY ? -INFINITY : m * f.sl2 - base);
-            m = mn;
-            float ls = 0.f;
+                    for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int j = 0; j < NK; ++j)
+                        for (int e = 0; e < 16; ++e) o[w][d][e] *= alpha[w];
+            }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e], f.sl2, -base));
-                    ls += s[j][e];
-                }
-            l = l * alpha + ls;
+            for (int w = 0; w < QW; ++w) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+                for (int i = 0; i < 2 * NK; ++i) {
+                    float x[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][i >> 1][8 * (i & 1) + e], f.sl2, -base[w]));
+                        l[w] += x[e];
+                    }
+                    Frag<NP> p;
+                    make_frag(x, p);
+                    if (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int i = 0; i < 2 * NK; ++i) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[i >> 1][8 * (i & 1) + e];
-                Frag<NP> p;
-                make_frag(x, p);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    Frag<NP> v;
-                    frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
-                    mma(o[d], v, p);
+                    for (int d = 0; d < ND; ++d) {
+                        Frag<NP> v;
+                        frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
+                        mma(o[w][d], v, p);
+                    }
+                    if (PRIO) __builtin_amdgcn_s_setprio(0);
                 }
             }
         }
@@ -159,33 +200,32 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(const fwd_params f) {
         __syncthreads();
     }
 
-    l = half_sum(l);
-    if (!live) return;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const float lse = l > 0.f ? m * f.sl2 + __builtin_amdgcn_logf(l) : -INFINITY;
-    const int64_t row = ((int64_t)b * a.H + head) * a.Tq + tq;
-    if (f.nsplit > 1) {
+#pragma unroll
+    for (int w = 0; w < QW; ++w) {
+        const float tot = half_sum(l[w]);
+        if (!live[w]) continue;
+        const float inv = tot > 0.f ? 1.f / tot : 0.f;
+        const float lse = tot > 0.f ? m[w] * f.sl2 + __builtin_amdgcn_logf(tot) : -INFINITY;
+        const int64_t row = ((int64_t)b * a.H + head[w]) * a.Tq + tq[w];
         const int64_t nrow = (int64_t)a.batch * a.H * a.Tq;
         float* po = f.po + (sp * nrow + row) * a.D;
+        T* op = (T*)a.o + b * a.o_b + tq[w] * a.o_t + head[w] * a.o_h;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int c = 32 * d + acc_row(e);
-                if (c < a.D) ctn_st4(po + c, f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv);
+                const f32x4 v = f32x4{o[w][d][e], o[w][d][e + 1], o[w][d][e + 2], o[w][d][e + 3]} * inv;
+                if (c < a.D) {
+                    if (f.nsplit > 1) ctn_st4(po + c, v);
+                    else store4(op + c, v);
+                }
             }
-        if (half == 0) f.pl[sp * nrow + row] = lse;
-        return;
-    }
-    T* op = (T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int c = 32 * d + acc_row(e);
-            if (c < a.D) store4(op + c, f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv);
+        if (half == 0) {
+            if (f.nsplit > 1) f.pl[sp * nrow + row] = lse;
+            else if (a.lse) a.lse[row] = lse;
         }
-    if (a.lse && half == 0) a.lse[row] = lse;
+    }
 }
 
 // Joins the key ranges of a row: o = sum_s 2^(l_s - max) o_s / sum_s 2^(l_s - max).  One wave per row, lanes along D.
@@ -222,7 +262,10 @@ template <typename T, int DT> constexpr int key_tile() { return Planes<T>::N * D
 
 // How the call is cut.  Packed: all query heads of a key head in one tile of at most 128 rows, where there are fewer than
 // 32 queries (a tile per head would leave most of its 32 rows empty and read the keys once per query head).
-struct fwd_cut { bool packed; int rows, nw, nqt, heads, nsplit; };
+struct fwd_cut { bool packed; int rows, nw, qw, nqt, heads, nsplit; };
+#ifndef QWF
+#define QWF 2
+#endif
 fwd_cut cut_forward(const ctn_attn_args& a) {
     fwd_cut c;
     const int G = a.H / a.Hk;
@@ -230,7 +273,8 @@ fwd_cut cut_forward(const ctn_attn_args& a) {
     c.rows = c.packed ? G * a.Tq : a.Tq;
     c.heads = c.packed ? a.Hk : a.H;
     c.nw = c.rows <= 32 ? 1 : c.rows <= 64 ? 2 : 4;
-    c.nqt = ctn_cdiv(c.rows, 32 * c.nw);
+    c.qw = c.nw == 4 && a.D <= 64 ? QWF : 1;
+    c.nqt = ctn_cdiv(c.rows, 32 * c.nw * c.qw);
     c.nsplit = 1;
     const int64_t blocks = (int64_t)a.batch * c.heads * c.nqt;
     const int tiles = ctn_cdiv(a.Tk, 64);
@@ -243,15 +287,15 @@ fwd_cut cut_forward(const ctn_attn_args& a) {
     return c;
 }
 
-template <typename T, int DT, int NW>
+template <typename T, int DT, int NW, int QW>
 void launch_fwd(const fwd_params& f, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, key_tile<T, DT>()>), dim3(grid), dim3(NW * 64), 0, s, f);
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, QW, key_tile<T, DT>()>), dim3(grid), dim3(NW * 64), 0, s, f);
 }
 template <typename T, int DT>
 void launch_fwd_nw(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
-    if (nw == 1) launch_fwd<T, DT, 1>(f, grid, s);
-    else if (nw == 2) launch_fwd<T, DT, 2>(f, grid, s);
-    else launch_fwd<T, DT, 4>(f, grid, s);
+    if (nw == 1) launch_fwd<T, DT, 1, 1>(f, grid, s);
+    else if (nw == 2) launch_fwd<T, DT, 2, 1>(f, grid, s);
+    else launch_fwd<T, DT, 4, DT == 128 ? 1 : QWF>(f, grid, s);
 }
 template <typename T>
 void launch_fwd_type(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
@@ -274,11 +318,11 @@ bool ctn_attn_args_ok(const ctn_attn_args* a, const char* who) {
     }
     const int es = a->type == CTN_TYPE_F32 ? 4 : 2;
     const bool some = a->batch > 0 && a->Tq > 0, keys = a->batch > 0 && a->Tk > 0;
-    if ((some && (!a->q || !attn::strides_ok(a->q, a->q_b, a->q_t, a->q_h, es) || !a->o ||
-                  !attn::strides_ok(a->o, a->o_b, a->o_t, a->o_h, es))) ||
-        (keys && (!a->k || !a->v || !attn::strides_ok(a->k, a->k_b, a->k_t, a->k_h, es) ||
-                  !attn::strides_ok(a->v, a->v_b, a->v_t, a->v_h, es)))) {
-        ctn_set_error("%s: q, k, v, o must be 16-byte aligned with strides of whole 16 bytes", who);
+    if ((some && (!a->q || !attn::strides_ok(a->q, a->q_b, a->q_t, a->q_h, es, a->D, a->Tq) || !a->o ||
+                  !attn::strides_ok(a->o, a->o_b, a->o_t, a->o_h, es, a->D, a->Tq))) ||
+        (keys && (!a->k || !a->v || !attn::strides_ok(a->k, a->k_b, a->k_t, a->k_h, es, a->D, a->Tk) ||
+                  !attn::strides_ok(a->v, a->v_b, a->v_t, a->v_h, es, a->D, a->Tk)))) {
+        ctn_set_error("%s: q, k, v, o must be 16-byte aligned with strides of whole 16 bytes and rows that do not overlap, less than 16 MiB apart", who);
         return false;
     }
     return true;

@@ -491,17 +491,18 @@ def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, 
 
 
 def _attn_operand(x, shape):
-    """x with unit feature stride, 16-byte aligned, all strides whole 16 bytes (itself or a dense copy), and its strides."""
+    """x with unit feature stride, 16-byte aligned, all strides whole 16 bytes, rows apart from each other by less than 16 MiB
+    (itself or a dense copy), and its strides."""
     b, t, h, d = x.stride()
-    m = 3 if x.dtype == torch.float32 else 7
-    if d != 1 or x.data_ptr() & 15 or (b | t | h) & m:
+    m, far = (3, 1 << 22) if x.dtype == torch.float32 else (7, 1 << 23)
+    if d != 1 or x.data_ptr() & 15 or (b | t | h) & m or not shape[3] <= t < far:
         if shape[0] == 1:
             b = 0
         if shape[1] == 1:
-            t = 0
+            t = shape[3]
         if shape[2] == 1:
             h = 0
-        if d != 1 or x.data_ptr() & 15 or (b | t | h) & m:
+        if d != 1 or x.data_ptr() & 15 or (b | t | h) & m or not shape[3] <= t < far:
             x = x.contiguous()
             t, h = shape[2] * shape[3], shape[3]
             b = shape[1] * t
@@ -537,9 +538,13 @@ def check_attention(q, k, v, lengths):
 @functools.lru_cache(maxsize=256)
 def _attn_ws(B, Tq, Tk, H, Hk, D, code, backward):
     """Workspace floats of a call of these sizes."""
-    a = _lib.AttnArgs(batch=B, Tq=Tq, Tk=Tk, H=H, Hk=Hk, D=D, type=code, scale=1.0, q=16, k=16, v=16, o=16)
+    a = _lib.AttnArgs(batch=B, Tq=Tq, Tk=Tk, H=H, Hk=Hk, D=D, type=code, scale=1.0, q=16, k=16, v=16, o=16, q_t=D, k_t=D, v_t=D,
+                      o_t=D)
     lib = _lib.load()
-    return max(0, (lib.ctn_attn_bwd_ws_floats if backward else lib.ctn_attn_fwd_ws_floats)(C.byref(a)))
+    need = (lib.ctn_attn_bwd_ws_floats if backward else lib.ctn_attn_fwd_ws_floats)(C.byref(a))
+    if need < 0:
+        _lib.check(need, "ctn_attn_ws_floats")
+    return need
 
 
 def _attn_lengths(lengths, Tk):
