@@ -21,12 +21,14 @@ template <typename T, int DT> constexpr int walk_tile() { return Planes<T>::N * 
 struct bwd_params {
     ctn_attn_args a;
     int G, nt;               // tiles of the kept axis per (batch element, head)
+    int nsplit;              // dK / dV: pieces of the walk over queries
     float sl2;
     float* delta;            // [B][H][Tq]
+    float* part;             // nsplit > 1: [nsplit][dk, dv][B][Tk][Hk][D]
 };
 
 template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const bwd_params f) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_dq_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, KT = walk_tile<T, DT>();
     typedef Tile<T, DT, KT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES;
@@ -34,10 +36,10 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const bwd_params f) {
     const ctn_attn_args& a = f.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
-    unsigned id = die_order(blockIdx.x, gridDim.x);
-    const int qt = f.nt - 1 - (int)(id % f.nt);
-    id /= f.nt;
-    const int head = id % a.H, b = id / a.H, hk = head / f.G;
+    unsigned tile, unit;
+    deal(blockIdx.x, a.batch * a.H, tile, unit);
+    const int qt = f.nt - 1 - (int)tile;                         // with a causal mask the last queries see the most keys
+    const int head = unit % a.H, b = unit / a.H, hk = head / f.G;
     const int w0 = qt * 32 * NW + wave * 32, tq = w0 + (lane & 31);
     const bool live = tq < a.Tq;
 
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const bwd_params f) {
 }
 
 template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2))) void attn_dkv_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
     typedef Tile<T, DT, QT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES + 2 * QT * 4;          // Q planes, dO planes, log-sums, deltas
@@ -168,10 +170,10 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
     const ctn_attn_args& a = f.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
-    unsigned id = die_order(blockIdx.x, gridDim.x);
-    const int kt = id % f.nt;                                    // with a causal mask the first keys are seen most
-    id /= f.nt;
-    const int hk = id % a.Hk, b = id / a.Hk;
+    unsigned tile, unit;
+    deal(blockIdx.x, a.batch * a.Hk, tile, unit);
+    const int sp = tile % f.nsplit, kt = tile / f.nsplit;        // with a causal mask the first keys are seen most
+    const int hk = unit % a.Hk, b = unit / a.Hk;
     const int b0 = kt * 32 * NW, w0 = b0 + wave * 32, key = w0 + (lane & 31);
 
     int len = a.Tk;
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
     const int wfull = w0 + 32 > len ? a.Tq : a.causal ? w0 + 31 - off : 0;
     const int t0 = first / QT;
     const int nq = b0 < len && a.Tq > first ? (a.Tq + QT - 1) / QT - t0 : 0;      // query tiles per head
-    const int ntile = nq * f.G;
+    const int i0 = (int)((int64_t)nq * f.G * sp / f.nsplit), i1 = (int)((int64_t)nq * f.G * (sp + 1) / f.nsplit);
 
     Frag<NP> k[KS], v[KS];
     {
@@ -233,16 +235,16 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
-    if (ntile > 0) {
-        fetch(0);
+    if (i0 < i1) {
+        fetch(i0);
         stage(0);
     }
     __syncthreads();
-    for (int i = 0; i < ntile; ++i) {
-        const unsigned char* Q = lds + (i & 1) * BUF;
+    for (int i = i0; i < i1; ++i) {
+        const unsigned char* Q = lds + ((i - i0) & 1) * BUF;
         const unsigned char* G = Q + tile_t::BYTES;
         const float* st = reinterpret_cast<const float*>(G + tile_t::BYTES);
-        if (i + 1 < ntile) fetch(i + 1);
+        if (i + 1 < i1) fetch(i + 1);
 #pragma unroll
         for (int r0 = 0; r0 < QT; r0 += 32) {
             const int q0 = (t0 + i % nq) * QT + r0;
@@ -294,23 +296,62 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const bwd_params f) {
                 }
             }
         }
-        if (i + 1 < ntile) stage((i + 1) & 1);
+        if (i + 1 < i1) stage((i - i0 + 1) & 1);
         __syncthreads();
     }
     if (key >= a.Tk) return;
     T* pk = (T*)a.dk + b * a.dk_b + key * a.dk_t + hk * a.dk_h;
     T* pv = (T*)a.dv + b * a.dv_b + key * a.dv_t + hk * a.dv_h;
+    const int64_t one = (int64_t)a.batch * a.Tk * a.Hk * a.D;
+    float* part = f.part + 2 * sp * one + (((int64_t)b * a.Tk + key) * a.Hk + hk) * a.D;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int c = 32 * d + acc_row(e);
             if (c >= a.D) continue;
-            if (a.dk) store4(pk + c, f32x4{dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]} * a.scale);
-            if (a.dv) store4(pv + c, f32x4{dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]});
+            const f32x4 x = f32x4{dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]} * a.scale;
+            const f32x4 y = f32x4{dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]};
+            if (f.nsplit > 1) {
+                ctn_st4(part + c, x);
+                ctn_st4(part + one + c, y);
+            } else {
+                if (a.dk) store4(pk + c, x);
+                if (a.dv) store4(pv + c, y);
+            }
         }
 }
 
+// Adds the pieces of a split walk, in their order: four elements of dk (blockIdx.y 0) or dv (1) per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_add_kernel(const bwd_params f) {
+    const ctn_attn_args& a = f.a;
+    const bool vals = blockIdx.y != 0;
+    if ((vals ? a.dv : a.dk) == nullptr) return;
+    const int64_t one = (int64_t)a.batch * a.Tk * a.Hk * a.D, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= one) return;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < f.nsplit; ++s) x += ctn_ld4(f.part + (2 * s + (vals ? 1 : 0)) * one + i);
+    const int d = i % a.D, hk = i / a.D % a.Hk;
+    const int64_t bt = i / a.D / a.Hk, t = bt % a.Tk, b = bt / a.Tk;
+    if (vals) store4((T*)a.dv + b * a.dv_b + t * a.dv_t + hk * a.dv_h + d, x);
+    else store4((T*)a.dk + b * a.dk_b + t * a.dk_t + hk * a.dk_h + d, x);
+}
+
+// Pieces of the dK / dV walk.  A launch of few blocks ends with its longest one -- a causal mask or few key heads under
+// many query heads make them unequal -- so the walk over (query head, query tile) is cut until there are two blocks a CU,
+// into pieces of four tiles at least.  4096 causal tokens, 16 heads on 4 of 128 features, bf16, two sequences (256 uncut
+// blocks): 1981 us uncut, 654 in two pieces, 677 in four (more sums to store and add).
+int dkv_pieces(const ctn_attn_args& a, const int nt) {
+    const int64_t blocks = (int64_t)a.batch * a.Hk * nt, tiles = (int64_t)(a.H / a.Hk) * ctn_cdiv(a.Tq, 64);
+    if (blocks >= 512) return 1;
+    int64_t n = (512 + blocks - 1) / blocks;
+    if (n > tiles / 4) n = tiles / 4;
+    return n < 1 ? 1 : n > 16 ? 16 : (int)n;
+}
+
+int64_t round16(const int64_t n) { return (n + 15) / 16 * 16; }
 int waves_for(const int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 
 template <typename T, int DT>
@@ -338,7 +379,8 @@ extern "C" {
 
 int64_t ctn_attn_bwd_ws_floats(const ctn_attn_args* a) {
     if (!ctn_attn_args_ok(a, "ctn_attn_bwd_ws_floats")) return -1;
-    return (int64_t)a->batch * a->H * a->Tq;
+    const int n = a->batch > 0 && a->Tk > 0 ? dkv_pieces(*a, ctn_cdiv(a->Tk, 32 * waves_for(a->Tk))) : 1;
+    return round16((int64_t)a->batch * a->H * a->Tq) + (n > 1 ? 2 * n * (int64_t)a->batch * a->Tk * a->Hk * a->D : 0);
 }
 
 int ctn_attn_bwd(const ctn_attn_args* a, void* stream) {
@@ -352,13 +394,16 @@ int ctn_attn_bwd(const ctn_attn_args* a, void* stream) {
                     (!a->dk || strides_ok(a->dk, a->dk_b, a->dk_t, a->dk_h, es, a->D, a->Tk)) &&
                     (!a->dv || strides_ok(a->dv, a->dv_b, a->dv_t, a->dv_h, es, a->D, a->Tk)),
                 "ctn_attn_bwd: dq, dk, dv must be 16-byte aligned with strides of whole 16 bytes");
-    CTN_REQUIRE(nrow == 0 || (a->ws && a->ws_floats >= nrow), "ctn_attn_bwd: workspace of %lld floats, %lld needed",
-                (long long)a->ws_floats, (long long)nrow);
+    const int64_t need = ctn_attn_bwd_ws_floats(a);
+    CTN_REQUIRE(need == 0 || (a->ws && ctn_aligned16(a->ws) && a->ws_floats >= need),
+                "ctn_attn_bwd: workspace of %lld floats, %lld needed", (long long)a->ws_floats, (long long)need);
     bwd_params f;
     f.a = *a;
     f.G = a->H / a->Hk;
     f.sl2 = a->scale * LOG2E;
     f.delta = a->ws;
+    f.part = a->ws + round16(nrow);
+    f.nsplit = 1;
     hipStream_t s = (hipStream_t)stream;
     if (a->Tq > 0) {                       // also where dq itself is not wanted: the second launch reads the deltas
         const int nw = waves_for(a->Tq);
@@ -372,11 +417,20 @@ int ctn_attn_bwd(const ctn_attn_args* a, void* stream) {
     if (a->Tk > 0 && (a->dk || a->dv)) {
         const int nw = waves_for(a->Tk);
         f.nt = ctn_cdiv(a->Tk, 32 * nw);
-        const int64_t grid = (int64_t)a->batch * a->Hk * f.nt;
+        f.nsplit = dkv_pieces(*a, f.nt);
+        const int64_t grid = (int64_t)a->batch * a->Hk * f.nt * f.nsplit;
+        const int64_t quads = ((int64_t)a->batch * a->Tk * a->Hk * a->D / 4 + 255) / 256;
         CTN_REQUIRE(grid < 0x7fffffff, "ctn_attn_bwd: too much work for one launch");
         if (a->type == CTN_TYPE_F32) launch_bwd<float>(true, f, nw, (unsigned)grid, s);
         else launch_bwd<__bf16>(true, f, nw, (unsigned)grid, s);
         CTN_CHECK_LAUNCH("ctn_attn_bwd (keys)");
+        if (f.nsplit > 1) {
+            CTN_REQUIRE(quads < 0x7fffffff, "ctn_attn_bwd: too much work for one launch");
+            const dim3 ag((unsigned)quads, 2);
+            if (a->type == CTN_TYPE_F32) hipLaunchKernelGGL(attn_add_kernel<float>, ag, dim3(256), 0, s, f);
+            else hipLaunchKernelGGL(attn_add_kernel<__bf16>, ag, dim3(256), 0, s, f);
+            CTN_CHECK_LAUNCH("ctn_attn_bwd (join)");
+        }
     }
     return CTN_OK;
 }

@@ -21,14 +21,8 @@ struct fwd_params {
     float* po; float* pl;                 // split: partial outputs [nsplit][B H Tq][D] and log2-sums [nsplit][B H Tq]
 };
 
-#ifndef WPE
-#define WPE 2
-#endif
-#ifndef PRIO
-#define PRIO 0
-#endif
 template <typename T, int DT, int NW, int QW, int KT>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) void attn_fwd_kernel(const fwd_params f) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_fwd_kernel(const fwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, NK = KT / 32, ND = DT / 32, ROWS = 32 * QW;
     typedef Tile<T, DT, KT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES;                       // a buffer: K planes, V planes
@@ -37,13 +31,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
 
-    // longest rows first: with a causal mask the last query tiles see the most keys
-    unsigned id = die_order(blockIdx.x, gridDim.x);
-    const int sp = id % f.nsplit;
-    id /= f.nsplit;
-    const int qt = f.nqt - 1 - (int)(id % f.nqt);
-    id /= f.nqt;
-    const int hh = id % f.heads, b = id / f.heads;
+    unsigned tile, unit;
+    deal(blockIdx.x, a.batch * f.heads, tile, unit);
+    const int sp = tile % f.nsplit;
+    const int qt = f.nqt - 1 - (int)(tile / f.nsplit);           // with a causal mask the last queries see the most keys
+    const int hh = unit % f.heads, b = unit / f.heads;
 
     const int w0 = (qt * NW + wave) * ROWS;                      // the wave's first row
     const int hk = f.packed ? hh : hh / f.G;
@@ -128,7 +120,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) 
                 for (int j = 0; j < NK; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[w][j][e] = 0.f;
-            if (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -138,7 +129,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) 
 #pragma unroll
                     for (int w = 0; w < QW; ++w) mma(s[w][j], k, q[w][i]);
                 }
-            if (PRIO) __builtin_amdgcn_s_setprio(0);
             if ((t + 1) * KT > wfull) {
 #pragma unroll
                 for (int w = 0; w < QW; ++w) {
@@ -185,14 +175,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) 
                     }
                     Frag<NP> p;
                     make_frag(x, p);
-                    if (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
                         Frag<NP> v;
                         frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
                         mma(o[w][d], v, p);
                     }
-                    if (PRIO) __builtin_amdgcn_s_setprio(0);
                 }
             }
         }
