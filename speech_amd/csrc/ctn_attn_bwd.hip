@@ -322,6 +322,259 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
         }
 }
 
+// ------------------------------------------------------------------------------------------------ one block per key head
+// Many short fp32 sequences with heads of up to 32 features (the dual-path blocks: thousands of (sequence, head) pairs of a
+// few hundred steps): one block of four waves owns a (batch element, key head) and forms all three gradients in five
+// products instead of the seven of the two launches above.  The walk is the dK / dV kernel's -- 128 keys at a time, 32 per
+// wave, over the query tiles of every head of the group -- and dQ comes out of the same score gradients: ds has the keys as
+// columns, dQ^T = K^T ds^T wants the queries there, and the matrix instruction itself turns it over, ds^T = ds^T I with ds
+// as the A operand (its register layout serves both operands alike) and the identity as B, exact on bf16 pieces, two
+// instructions a piece.  The four waves' dQ tiles meet in LDS, in the waves' order, behind the one barrier of a tile, and the
+// sums leave while the next tile's products run; later key blocks add to what the block's own threads stored in dq.  delta
+// is formed where dO is staged.  66 matrix instructions per 32 x 32 scores (the two launches: 84, with twice the exponentials).
+// For bf16 tensors, six times fewer matrix instructions, the two launches are faster (2000 sequence heads of 250 steps,
+// D = 32: 135 us against 188 us).
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_bwd_whole_kernel(const bwd_params f) {
+    constexpr int NP = 3, DT = 32, PLANE = 32 * DT * 2, TILE = NP * PLANE, BUF = 2 * TILE + 256, DQ = 4 * 32 * DT;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 2 * DQ * 4];
+    float* const dqs = reinterpret_cast<float*>(lds + 2 * BUF);          // two buffers of [4 waves][32 queries][32]
+    const ctn_attn_args& a = f.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
+    const int off = a.Tk - a.Tq, D = a.D, Tq = a.Tq, G = f.G;
+    const bool causal = a.causal != 0;
+    const float sl2 = f.sl2, scale = a.scale;
+    unsigned tile0, unit;
+    deal(blockIdx.x, gridDim.x, tile0, unit);
+    const int hk = unit % a.Hk, b = unit / a.Hk;
+    int len = a.Tk;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
+    const int nkb = (a.Tk + 127) / 128;
+
+    Frag<1> eye[2];                                              // identity, rows in the accumulators' order
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) eye[j].p[0][i] = (__bf16)(16 * j + 4 * half + (i & 3) + 8 * (i >> 2) == l31 ? 1.f : 0.f);
+
+    // staging: waves 0 and 1 carry the query tile, 2 and 3 the tile of output gradients and of outputs; a thread has chunk
+    // (row, ch) of eight features
+    const bool grad = wave >= 2;
+    const int row = (tid & 127) >> 2, ch = tid & 3;
+    const int64_t st_ = grad ? a.do_t : a.q_t, sh_ = grad ? a.do_h : a.q_h;
+    const float* const sbase = (grad ? (const float*)a.d_o + b * a.do_b : (const float*)a.q + b * a.q_b) + (int64_t)hk * G * sh_;
+    const float* const obase = (const float*)a.o + b * a.o_b + (int64_t)hk * G * a.o_h;
+    const float* const lbase = a.lse + ((int64_t)b * a.H + hk * G) * Tq;
+    const int pitch = (int)st_ * 4, opitch = (int)a.o_t * 4;
+    const int voff = ch * 8 < D ? row * pitch + ch * 32 : 0x7fffff00, ooff = ch * 8 < D ? row * opitch + ch * 32 : 0x7fffff00;
+    u32x4 c0, c1, o0, o1;
+    float lse = 0.f;
+    const float* sp = sbase;                                     // the next tile to fetch: its rows, and where it stands
+    const float* op = obase;
+    int fg = 0, fq = 0;
+    auto seek = [&](const int g, const int q0) {
+        fg = g, fq = q0;
+        sp = sbase + g * sh_ + q0 * st_;
+        op = obase + g * a.o_h + q0 * a.o_t;
+    };
+    auto fetch = [&](const int tfirst) {
+        const int rows = min(Tq - fq, 32);
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)sp, 0, (rows - 1) * pitch + D * 4, 0x00020000);
+        c0 = __builtin_amdgcn_raw_buffer_load_b128(rs, voff, 0, 0);
+        c1 = __builtin_amdgcn_raw_buffer_load_b128(rs, voff + 16, 0, 0);
+        if (grad) {
+            const auto ro = __builtin_amdgcn_make_buffer_rsrc((void*)op, 0, (rows - 1) * opitch + D * 4, 0x00020000);
+            o0 = __builtin_amdgcn_raw_buffer_load_b128(ro, ooff, 0, 0);
+            o1 = __builtin_amdgcn_raw_buffer_load_b128(ro, ooff + 16, 0, 0);
+        } else if (tid < 32) {
+            lse = tid < rows ? lbase[(int64_t)fg * Tq + fq + tid] : INFINITY;
+            if (lse == -INFINITY) lse = INFINITY;                // sees nothing: every probability comes out as zero
+        }
+        fq += 32, sp += 32 * st_, op += 32 * a.o_t;
+        if (fq >= Tq) seek(fg + 1, tfirst);
+    };
+    auto stage = [&](const int buf) {
+        unsigned char* p = lds + buf * BUF;
+        float* st = reinterpret_cast<float*>(p + 2 * TILE);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(c0[i]), x[4 + i] = __uint_as_float(c1[i]);
+        Frag<NP> fr;
+        make_frag(x, fr);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(p + (grad ? TILE : 0) + n * PLANE + img<DT>(row, ch)) = fr.p[n];
+        if (grad) {
+            float d = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d += x[i] * __uint_as_float(o0[i]) + x[4 + i] * __uint_as_float(o1[i]);
+            d += __shfl_xor(d, 1);
+            d += __shfl_xor(d, 2);
+            if (ch == 0) st[32 + row] = d;
+        } else if (tid < 32) {
+            st[tid] = lse;
+        }
+    };
+
+    // dq: a thread sums four features of one query of a tile
+    const int dr = tid >> 3, dd = (tid & 7) * 4;
+    float* const dqbase = (float*)a.dq + b * a.dq_b + (int64_t)hk * G * a.dq_h + dd;
+    // queries in front of the first tile that sees a key (all of them, if none does) have no gradient
+    if (a.dq != nullptr && dd < D) {
+        const int dead = len > 0 ? (causal ? min(max(0, -off) / 32 * 32, Tq) : 0) : Tq;
+        for (int g = 0; g < G; ++g)
+            for (int t = dr; t < dead; t += 32) ctn_st4(dqbase + g * a.dq_h + t * a.dq_t, f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+
+    for (int kb = 0; kb < nkb; ++kb) {
+        const int b0 = kb * 128, w0 = b0 + wave * 32, key = w0 + l31;
+        const bool seen = key < len;
+        // query q sees key j when j <= q + off: block's and wave's first query, and the wave's first query without a mask
+        const int first = causal ? max(0, b0 - off) : 0, wfirst = causal ? max(0, w0 - off) : 0;
+        const int wfull = w0 + 32 > len ? Tq : causal ? w0 + 31 - off : 0;
+        const int q1 = first / 32 * 32;                          // first query of the walk
+        const int ntile = b0 < len && Tq > first ? ((Tq + 31) / 32 - q1 / 32) * G : 0;
+
+        __syncthreads();                                         // dqs and the tile buffers are free
+        Frag<NP> k[2], v[2], kt[2];                              // keys, values; the keys' columns
+        {
+            const float* kp = (const float*)a.k + b * a.k_b + key * a.k_t + hk * a.k_h;
+            const float* vp = (const float*)a.v + b * a.v_b + key * a.v_t + hk * a.v_h;
+            unsigned char* own = lds + 2 * BUF + wave * TILE;    // this wave's, read back before anything else comes here
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int d = 16 * s + 8 * half;
+                Chunk<float> ck, cv;
+                if (seen && d < D) ck.load(kp + d), cv.load(vp + d);
+                else ck.zero(), cv.zero();
+                ck.frag(k[s]);
+                cv.frag(v[s]);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(own + n * PLANE + img<DT>(l31, 2 * s + half)) = k[s].p[n];
+            }
+            if (ntile > 0) {
+                seek(0, q1);
+                fetch(q1);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) frag_cols<NP, DT, 32>(own, 16 * j, 0, kt[j]);
+        }
+        f32x16 dk, dv;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[e] = dv[e] = 0.f;
+        if (ntile > 0) stage(0);
+        __syncthreads();
+        int q0 = q1, g = 0;
+        float* dp = dqbase + (q0 + dr) * a.dq_t;
+        for (int i = 0; i < ntile; ++i) {
+            const unsigned char* Q = lds + (i & 1) * BUF;
+            const unsigned char* GO = Q + TILE;
+            const float* st = reinterpret_cast<const float*>(GO + TILE);
+            const bool out = a.dq != nullptr && q0 + dr < Tq && dd < D;
+            if (i + 1 < ntile) fetch(q1);
+            f32x4 before = {0.f, 0.f, 0.f, 0.f};                 // what earlier key blocks left
+            if (kb > 0 && out) before = ctn_ld4(dp);
+            f32x16 dq;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dq[e] = 0.f;
+            if (q0 + 32 > wfirst && w0 < len) {
+                f32x16 s, p;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = p[e] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    Frag<NP> x;
+                    frag_rows<NP, DT, 32>(Q, 0, j, x);
+                    mma(s, x, k[j]);
+                    frag_rows<NP, DT, 32>(GO, 0, j, x);
+                    mma(p, x, v[j]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 ls = ctn_ld4(st + 8 * r + 4 * half), delta = ctn_ld4(st + 32 + 8 * r + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * r + e], sl2, -ls[e]));
+                        s[4 * r + e] = w;
+                        p[4 * r + e] = w * (p[4 * r + e] - delta[e]);
+                    }
+                }
+                if (q0 < wfull) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const bool on = seen && (!causal || key <= q0 + acc_row(e) + off);
+                        s[e] = on ? s[e] : 0.f;
+                        p[e] = on ? p[e] : 0.f;
+                    }
+                }
+                Frag<NP> ds[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = s[8 * j + e];
+                    Frag<NP> w, y;
+                    make_frag(x, w);
+                    frag_cols<NP, DT, 32>(GO, 16 * j, 0, y);
+                    mma(dv, y, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = p[8 * j + e];
+                    make_frag(x, ds[j]);
+                    frag_cols<NP, DT, 32>(Q, 16 * j, 0, y);
+                    mma(dk, y, ds[j]);
+                }
+                Frag<NP> dt[2];                                  // ds with the queries as columns
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    f32x16 x;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ds[j].p[n], eye[j].p[0], x, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = x[8 * j + e];
+                        Frag<1> z;
+                        make_frag(y, z);                         // exact: the values are bf16 ones
+                        dt[j].p[n] = z.p[0];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma(dq, kt[j], dt[j]);
+            }
+            // [wave][query][feature], the 16-byte chunks of a row turned by the query so that a column's lanes spread over the banks
+            float* part = dqs + (i & 1) * DQ;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                ctn_st4(part + (32 * wave + l31) * DT + 4 * ((acc_row(e) >> 2) ^ (l31 & 7)), f32x4{dq[e], dq[e + 1], dq[e + 2], dq[e + 3]});
+            if (i + 1 < ntile) stage((i + 1) & 1);
+            // behind this barrier tile i + 1 and the partial dq of tile i are in LDS; the buffers written next were last read
+            // in front of it
+            __syncthreads();
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x += ctn_ld4(part + (32 * w + dr) * DT + 4 * ((dd >> 2) ^ (dr & 7)));
+            if (out) ctn_st4(dp, before + x * scale);
+            q0 += 32, dp += 32 * a.dq_t;
+            if (q0 >= Tq) {
+                q0 = q1, ++g;
+                dp = dqbase + g * a.dq_h + (q0 + dr) * a.dq_t;
+            }
+        }
+        if (key < a.Tk) {
+            float* pk = (float*)a.dk + b * a.dk_b + key * a.dk_t + hk * a.dk_h;
+            float* pv = (float*)a.dv + b * a.dv_b + key * a.dv_t + hk * a.dv_h;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int cc = acc_row(e);
+                if (cc >= D) continue;
+                if (a.dk) ctn_st4(pk + cc, f32x4{dk[e], dk[e + 1], dk[e + 2], dk[e + 3]} * scale);
+                if (a.dv) ctn_st4(pv + cc, f32x4{dv[e], dv[e + 1], dv[e + 2], dv[e + 3]});
+            }
+        }
+    }
+}
+
 // Adds the pieces of a split walk, in their order: four elements of dk (blockIdx.y 0) or dv (1) per thread.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_add_kernel(const bwd_params f) {
@@ -349,6 +602,11 @@ int dkv_pieces(const ctn_attn_args& a, const int nt) {
     int64_t n = (512 + blocks - 1) / blocks;
     if (n > tiles / 4) n = tiles / 4;
     return n < 1 ? 1 : n > 16 ? 16 : (int)n;
+}
+
+// One block per key head: where there are four blocks a CU at least.
+bool whole_fits(const ctn_attn_args& a) {
+    return a.type == CTN_TYPE_F32 && a.D <= 32 && (int64_t)a.batch * a.Hk >= 1024 && a.Tq > 0 && a.Tk > 0;
 }
 
 int64_t round16(const int64_t n) { return (n + 15) / 16 * 16; }
@@ -379,6 +637,7 @@ extern "C" {
 
 int64_t ctn_attn_bwd_ws_floats(const ctn_attn_args* a) {
     if (!ctn_attn_args_ok(a, "ctn_attn_bwd_ws_floats")) return -1;
+    if (whole_fits(*a)) return 0;
     const int n = a->batch > 0 && a->Tk > 0 ? dkv_pieces(*a, ctn_cdiv(a->Tk, 32 * waves_for(a->Tk))) : 1;
     return round16((int64_t)a->batch * a->H * a->Tq) + (n > 1 ? 2 * n * (int64_t)a->batch * a->Tk * a->Hk * a->D : 0);
 }
@@ -405,6 +664,13 @@ int ctn_attn_bwd(const ctn_attn_args* a, void* stream) {
     f.part = a->ws + round16(nrow);
     f.nsplit = 1;
     hipStream_t s = (hipStream_t)stream;
+    if (whole_fits(*a)) {
+        const int64_t grid = (int64_t)a->batch * a->Hk;
+        CTN_REQUIRE(grid < 0x7fffffff, "ctn_attn_bwd: too much work for one launch");
+        hipLaunchKernelGGL(attn_bwd_whole_kernel, dim3((unsigned)grid), dim3(256), 0, s, f);
+        CTN_CHECK_LAUNCH("ctn_attn_bwd (whole heads)");
+        return CTN_OK;
+    }
     if (a->Tq > 0) {                       // also where dq itself is not wanted: the second launch reads the deltas
         const int nw = waves_for(a->Tq);
         f.nt = ctn_cdiv(a->Tq, 32 * nw);

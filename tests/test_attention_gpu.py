@@ -211,6 +211,42 @@ def test_attention_split_over_keys(B, Tq, Tk, H, Hk, D, causal, lengths, dtype):
         ref.check(a, b, t, n)
 
 
+#         B, Tq,  Tk,  H, Hk, D, causal, ragged
+MANY = [(1024, 33, 33, 1, 1, 32, False, False), (300, 40, 40, 8, 4, 32, True, True), (520, 20, 70, 2, 2, 8, True, True),
+        (520, 70, 20, 2, 2, 24, True, False), (260, 150, 150, 4, 4, 32, True, True), (128, 40, 300, 16, 8, 16, True, True),
+        (1024, 1, 129, 1, 1, 32, False, True), (128, 129, 257, 8, 8, 32, False, False), (1030, 5, 3, 1, 1, 16, True, False),
+        (512, 100, 40, 4, 2, 64, True, True), (256, 33, 200, 4, 4, 56, False, True), (1024, 35, 300, 2, 1, 40, True, True)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,causal,ragged", MANY)
+def test_attention_of_many_sequences(B, Tq, Tk, H, Hk, D, causal, ragged, dtype):
+    """Enough (sequence, key head) pairs for the backward pass that gives each one a block, within one key block and over
+    several, lengths of zero among them."""
+    fused = normal((B, max(Tq, Tk), H + 2 * Hk, D), 1, dtype)
+    q, k, v = fused[:, :Tq, :H], fused[:, :Tk, H:H + Hk], fused[:, :Tk, H + Hk:]
+    do = normal((B, Tq, H, D), 4, dtype)
+    lens = None
+    if ragged:
+        lens = torch.randint(0, Tk + 1, (B,), generator=torch.Generator().manual_seed(5))
+        lens[:2] = torch.tensor([0, Tk])
+        for b in range(B):
+            fused[b, lens[b]:, H:] = math.nan if b % 2 else math.inf
+    fd = fused.to(DEV)
+    leaves = [fd[:, :Tq, :H].requires_grad_(True), fd[:, :Tk, H:H + Hk].requires_grad_(True),
+              fd[:, :Tk, H + Hk:].requires_grad_(True)]
+
+    def run():
+        o = attention(*leaves, lengths=None if lens is None else lens.to(DEV), causal=causal)
+        return [o.detach()] + list(torch.autograd.grad(o, leaves, do.to(DEV)))
+
+    got = run()
+    want, bound = ref.attention(q, k, v, lens, causal, do=do)
+    for n, a, b, t in zip(("o", "dq", "dk", "dv"), got, want, bound):
+        ref.check(a, b, t, n)
+    assert all(torch.equal(a, b) for a, b in zip(got, run()))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_reads_nothing_behind_a_length(dtype):
     q, k, v, do = (normal((2, 50, 2, 32), i, dtype) for i in range(4))
