@@ -201,19 +201,20 @@ __device__ __forceinline__ void store4(__bf16* p, const f32x4 v) {
     *reinterpret_cast<unsigned long long*>(p) = x.u;
 }
 
-// Block index -> (tile, unit), unit = a (batch element, head): tile by tile over all units, so that with a causal mask the
-// long tiles of every unit start before the short ones (the other order ends with a long tail: 49 against 33 tile times at
-// 32 tiles, four units a die).  Blocks are dealt to the eight dies in turn; where the units divide by eight every die keeps
-// its own ones, whose keys then stay in its L2.
-__device__ __forceinline__ void deal(const unsigned id, const unsigned units, unsigned& tile, unsigned& unit) {
-    if ((units & 7u) == 0) {
-        const unsigned per = units >> 3, i = id >> 3;
-        tile = i / per;
-        unit = (id & 7u) * per + (i - tile * per);
-    } else {
-        tile = id / units;
-        unit = id - tile * units;
-    }
+// Block index -> (tile, unit), unit = a (batch element, head), `per` tiles each.  Blocks are dealt to the eight dies in turn;
+// where the units divide by eight every die keeps its own ones, whose keys then stay in its L2.  Within a die the tiles of
+// a unit follow each other; with a causal mask they run tile by tile over as many units as make 128 blocks, so that the long tiles
+// start before the short ones (unit by unit 32 tiles of four units a die end with a tail: 49 against 33 tile times) and
+// a unit's keys are still read close together.
+__device__ __forceinline__ void deal(const unsigned id, const unsigned units, const unsigned per, const bool causal, unsigned& tile,
+                                     unsigned& unit) {
+    const unsigned dies = (units & 7u) == 0 ? 8 : 1, mine = units / dies;
+    const unsigned die = dies == 8 ? id & 7u : 0, i = dies == 8 ? id >> 3 : id;
+    const unsigned group = causal ? (128 * (8 / dies) + per - 1) / per : 1;
+    const unsigned gi = i / (group * per), r = i - gi * group * per;
+    const unsigned left = mine - gi * group, here = left < group ? left : group;
+    tile = r / here;
+    unit = die * mine + gi * group + (r - tile * here);
 }
 
 // 16-byte aligned, strides of whole 16 bytes; rows (of D elements, T of them) that do not overlap and lie less than

@@ -21,44 +21,36 @@ struct fwd_params {
     float* po; float* pl;                 // split: partial outputs [nsplit][B H Tq][D] and log2-sums [nsplit][B H Tq]
 };
 
-template <typename T, int DT, int NW, int QW, int KT>
+template <typename T, int DT, int NW, int KT>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_fwd_kernel(const fwd_params f) {
-    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, NK = KT / 32, ND = DT / 32, ROWS = 32 * QW;
+    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, NK = KT / 32, ND = DT / 32;
     typedef Tile<T, DT, KT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES;                       // a buffer: K planes, V planes
     __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
     const ctn_attn_args& a = f.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
-
     unsigned tile, unit;
-    deal(blockIdx.x, a.batch * f.heads, tile, unit);
+    deal(blockIdx.x, a.batch * f.heads, f.nqt * f.nsplit, a.causal, tile, unit);
     const int sp = tile % f.nsplit;
     const int qt = f.nqt - 1 - (int)(tile / f.nsplit);           // with a causal mask the last queries see the most keys
     const int hh = unit % f.heads, b = unit / f.heads;
 
-    const int w0 = (qt * NW + wave) * ROWS;                      // the wave's first row
-    const int hk = f.packed ? hh : hh / f.G;
+    const int w0 = (qt * NW + wave) * 32;                        // the wave's first row
+    const int n = w0 + (lane & 31);
+    const bool live = n < f.rows;
+    const int g = f.packed ? n / a.Tq : 0, tq = f.packed ? n - g * a.Tq : n;
+    const int hk = f.packed ? hh : hh / f.G, head = f.packed ? hh * f.G + g : hh;
     int len = a.Tk;
     if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
-    int vis[QW], tq[QW], head[QW];                               // keys 0 .. vis - 1 are visible to the lane's rows
-    bool live[QW];
-#pragma unroll
-    for (int w = 0; w < QW; ++w) {
-        const int n = w0 + 32 * w + (lane & 31);
-        live[w] = n < f.rows;
-        const int g = f.packed ? n / a.Tq : 0;
-        tq[w] = f.packed ? n - g * a.Tq : n;
-        head[w] = f.packed ? hh * f.G + g : hh;
-        vis[w] = !live[w] ? 0 : a.causal ? min(len, tq[w] + off + 1) : len;
-    }
+    const int vis = !live ? 0 : a.causal ? min(len, tq + off + 1) : len;         // keys 0 .. vis - 1 are visible
     // block: keys below kend are read; wave: tiles below wfull need no mask, tiles from wend on hold nothing for it
     int kend = len, wfull = len, wend = len;
     if (a.causal) {
-        const int last = f.packed ? a.Tq - 1 : min(f.rows, (qt + 1) * ROWS * NW) - 1;
+        const int last = f.packed ? a.Tq - 1 : min(f.rows, (qt + 1) * 32 * NW) - 1;
         kend = min(len, last + off + 1);
         wfull = min(len, (f.packed ? 0 : w0) + off + 1);
-        wend = min(len, (f.packed ? a.Tq : min(f.rows, w0 + ROWS)) + off);
+        wend = min(len, (f.packed ? a.Tq : min(f.rows, w0 + 32)) + off);
     }
     if (w0 >= f.rows) wend = 0;
     const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
@@ -82,29 +74,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     };
     if (t0 < t1) fetch();
 
-    Frag<NP> q[QW][KS];
-#pragma unroll
-    for (int w = 0; w < QW; ++w) {
-        const T* qp = (const T*)a.q + b * a.q_b + tq[w] * a.q_t + head[w] * a.q_h;
+    Frag<NP> q[KS];
+    {
+        const T* qp = (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             Chunk<T> c;
             const int d = 16 * s + 8 * half;
-            if (live[w] && d < a.D) c.load(qp + d);
+            if (live && d < a.D) c.load(qp + d);
             else c.zero();
-            c.frag(q[w][s]);
+            c.frag(q[s]);
         }
     }
-    f32x16 o[QW][ND];
-    float m[QW], l[QW];
+    f32x16 o[ND];
 #pragma unroll
-    for (int w = 0; w < QW; ++w) {
-        m[w] = -INFINITY, l[w] = 0.f;
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[w][d][e] = 0.f;
-    }
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
 
     if (t0 < t1) stage(0);
     __syncthreads();
@@ -113,74 +100,57 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         const unsigned char* V = K + tile_t::BYTES;
         if (t + 1 < t1) fetch();
         if (t * KT < wend) {
-            f32x16 s[QW][NK];
+            f32x16 s[NK];
 #pragma unroll
-            for (int w = 0; w < QW; ++w)
+            for (int j = 0; j < NK; ++j)
 #pragma unroll
-                for (int j = 0; j < NK; ++j)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[w][j][e] = 0.f;
+                for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i)
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
                     Frag<NP> k;
                     frag_rows<NP, DT, KT>(K, 32 * j, i, k);
-#pragma unroll
-                    for (int w = 0; w < QW; ++w) mma(s[w][j], k, q[w][i]);
+                    mma(s[j], k, q[i]);
                 }
             if ((t + 1) * KT > wfull) {
-#pragma unroll
-                for (int w = 0; w < QW; ++w) {
-                    const int lim = vis[w] - t * KT - 4 * half;
-#pragma unroll
-                    for (int j = 0; j < NK; ++j)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[w][j][e] = 32 * j + (e & 3) + 8 * (e >> 2) < lim ? s[w][j][e] : -INFINITY;
-                }
-            }
-            float base[QW], alpha[QW];
-            bool moved = false;
-#pragma unroll
-            for (int w = 0; w < QW; ++w) {
-                float mx = s[w][0][0];
+                const int lim = vis - t * KT - 4 * half;
 #pragma unroll
                 for (int j = 0; j < NK; ++j)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[w][j][e]);
-                const float mn = fmaxf(m[w], half_max(mx));
-                base[w] = mn == -INFINITY ? 0.f : mn * f.sl2;    // rows that see nothing yet stay at zero
-                alpha[w] = __builtin_amdgcn_exp2f(m[w] * f.sl2 - base[w]);
-                moved |= mn != m[w];
-                m[w] = mn;
-                l[w] *= alpha[w];
+                    for (int e = 0; e < 16; ++e) s[j][e] = 32 * j + (e & 3) + 8 * (e >> 2) < lim ? s[j][e] : -INFINITY;
             }
-            if (__any(moved)) {
+            float mx = s[0][0];
 #pragma unroll
-                for (int w = 0; w < QW; ++w)
+            for (int j = 0; j < NK; ++j)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[j][e]);
+            const float mn = fmaxf(m, half_max(mx));
+            const float base = mn == -INFINITY ? 0.f : mn * f.sl2;           // rows that see nothing yet stay at zero
+            if (__any(mn != m)) {
+                const float alpha = __builtin_amdgcn_exp2f(m * f.sl2 - base);
+                l *= alpha;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[w][d][e] *= alpha[w];
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
             }
+            m = mn;
 #pragma unroll
-            for (int w = 0; w < QW; ++w) {
+            for (int i = 0; i < 2 * NK; ++i) {
+                float x[8];
 #pragma unroll
-                for (int i = 0; i < 2 * NK; ++i) {
-                    float x[8];
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], f.sl2, -base));
+                    l += x[e];
+                }
+                Frag<NP> p;
+                make_frag(x, p);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][i >> 1][8 * (i & 1) + e], f.sl2, -base[w]));
-                        l[w] += x[e];
-                    }
-                    Frag<NP> p;
-                    make_frag(x, p);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        Frag<NP> v;
-                        frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
-                        mma(o[w][d], v, p);
-                    }
+                for (int d = 0; d < ND; ++d) {
+                    Frag<NP> v;
+                    frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
+                    mma(o[d], v, p);
                 }
             }
         }
@@ -188,31 +158,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         __syncthreads();
     }
 
+    l = half_sum(l);
+    if (!live) return;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float lse = l > 0.f ? m * f.sl2 + __builtin_amdgcn_logf(l) : -INFINITY;
+    const int64_t row = ((int64_t)b * a.H + head) * a.Tq + tq, nrow = (int64_t)a.batch * a.H * a.Tq;
+    float* po = f.po + (sp * nrow + row) * a.D;
+    T* op = (T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h;
 #pragma unroll
-    for (int w = 0; w < QW; ++w) {
-        const float tot = half_sum(l[w]);
-        if (!live[w]) continue;
-        const float inv = tot > 0.f ? 1.f / tot : 0.f;
-        const float lse = tot > 0.f ? m[w] * f.sl2 + __builtin_amdgcn_logf(tot) : -INFINITY;
-        const int64_t row = ((int64_t)b * a.H + head[w]) * a.Tq + tq[w];
-        const int64_t nrow = (int64_t)a.batch * a.H * a.Tq;
-        float* po = f.po + (sp * nrow + row) * a.D;
-        T* op = (T*)a.o + b * a.o_b + tq[w] * a.o_t + head[w] * a.o_h;
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int c = 32 * d + acc_row(e);
-                const f32x4 v = f32x4{o[w][d][e], o[w][d][e + 1], o[w][d][e + 2], o[w][d][e + 3]} * inv;
-                if (c < a.D) {
-                    if (f.nsplit > 1) ctn_st4(po + c, v);
-                    else store4(op + c, v);
-                }
+        for (int e = 0; e < 16; e += 4) {
+            const int c = 32 * d + acc_row(e);
+            const f32x4 v = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv;
+            if (c < a.D) {
+                if (f.nsplit > 1) ctn_st4(po + c, v);
+                else store4(op + c, v);
             }
-        if (half == 0) {
-            if (f.nsplit > 1) f.pl[sp * nrow + row] = lse;
-            else if (a.lse) a.lse[row] = lse;
         }
+    if (half == 0) {
+        if (f.nsplit > 1) f.pl[sp * nrow + row] = lse;
+        else if (a.lse) a.lse[row] = lse;
     }
 }
 
@@ -245,15 +211,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const fwd_params f) {
     if (a.lse && lane == 0) a.lse[row] = tot > 0.f ? mx + __builtin_amdgcn_logf(tot) : -INFINITY;
 }
 
-// keys per tile: 64, halved where three planes of 128 features would take more than the LDS gives two buffers of
-template <typename T, int DT> constexpr int key_tile() { return Planes<T>::N * DT > 192 ? 32 : 64; }
+// Keys per tile: 64, halved where the LDS of three planes would keep a third block off the CU (fp32 heads of 64 features,
+// 16 x 8 heads of 1000 steps: 183 us against 222 us; of 32: 510 us against 535 us the other way) or the blocks are small.
+template <typename T, int DT, int NW> constexpr int key_tile() {
+    return Planes<T>::N * DT > 128 || (Planes<T>::N == 3 && NW < 4) ? 32 : 64;
+}
 
 // How the call is cut.  Packed: all query heads of a key head in one tile of at most 128 rows, where there are fewer than
 // 32 queries (a tile per head would leave most of its 32 rows empty and read the keys once per query head).
-struct fwd_cut { bool packed; int rows, nw, qw, nqt, heads, nsplit; };
-#ifndef QWF
-#define QWF 2
-#endif
+struct fwd_cut { bool packed; int rows, nw, nqt, heads, nsplit; };
 fwd_cut cut_forward(const ctn_attn_args& a) {
     fwd_cut c;
     const int G = a.H / a.Hk;
@@ -261,8 +227,7 @@ fwd_cut cut_forward(const ctn_attn_args& a) {
     c.rows = c.packed ? G * a.Tq : a.Tq;
     c.heads = c.packed ? a.Hk : a.H;
     c.nw = c.rows <= 32 ? 1 : c.rows <= 64 ? 2 : 4;
-    c.qw = c.nw == 4 && a.D <= 64 ? QWF : 1;
-    c.nqt = ctn_cdiv(c.rows, 32 * c.nw * c.qw);
+    c.nqt = ctn_cdiv(c.rows, 32 * c.nw);
     c.nsplit = 1;
     const int64_t blocks = (int64_t)a.batch * c.heads * c.nqt;
     const int tiles = ctn_cdiv(a.Tk, 64);
@@ -275,15 +240,15 @@ fwd_cut cut_forward(const ctn_attn_args& a) {
     return c;
 }
 
-template <typename T, int DT, int NW, int QW>
+template <typename T, int DT, int NW>
 void launch_fwd(const fwd_params& f, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, QW, key_tile<T, DT>()>), dim3(grid), dim3(NW * 64), 0, s, f);
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, key_tile<T, DT, NW>()>), dim3(grid), dim3(NW * 64), 0, s, f);
 }
 template <typename T, int DT>
 void launch_fwd_nw(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
-    if (nw == 1) launch_fwd<T, DT, 1, 1>(f, grid, s);
-    else if (nw == 2) launch_fwd<T, DT, 2, 1>(f, grid, s);
-    else launch_fwd<T, DT, 4, DT == 128 ? 1 : QWF>(f, grid, s);
+    if (nw == 1) launch_fwd<T, DT, 1>(f, grid, s);
+    else if (nw == 2) launch_fwd<T, DT, 2>(f, grid, s);
+    else launch_fwd<T, DT, 4>(f, grid, s);
 }
 template <typename T>
 void launch_fwd_type(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
