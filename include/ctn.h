@@ -267,12 +267,15 @@ int ctn_rotary(const void* x, int64_t xbs, int64_t xts, int64_t xhs, int B, int 
 /* ctn_attn_*: o[b][i][h] = sum_j p_ij v[b][j][h / (H / Hk)], p = softmax over the visible keys of scale q_i . k_j.  Key j is
  * visible to query i when j < lengths[b] (int32, clamped to 0 .. Tk; null: Tk) and, if causal, j <= i + Tk - Tq (the last
  * query sees the last key).  A row that sees no key is zero and has zero gradients.  Keys and values at or behind
- * lengths[b] are never read; a causal mask hides scores only: a NaN or infinity in v (or k, in the backward pass) behind a query's last key but
- * before lengths[b] may reach it.
+ * lengths[b] are never read; a causal mask hides scores only: a NaN or infinity in v (or k, in the backward pass) behind a
+ * query's last key but before lengths[b] may reach it, and one in a query's d_o the gradients of its neighbours.
  * q, o, d_o, dq (batch, Tq, H, D), k, v, dk, dv (batch, Tk, Hk, D) by strides (batch, token, head) with unit feature stride,
  * 16-byte aligned, strides multiples of 16 bytes; D a multiple of 8 up to 128, H a multiple of Hk, scale > 0.
  * lse (batch, H, Tq) floats: log2 of the row's sum of exp(score), -infinity for a row that sees nothing; may be null in the
  * forward call, read by the backward call, which recomputes the probabilities from it.
+ * o_low: for bf16 calls, what the rounding of o left over, in bf16 and laid out as o (may be null).  Written by the forward
+ * call, read by the backward call next to o: the row sums of d_o . o then are as exact as the forward pass's own sums, which the
+ * score gradients of rows that see few keys need.
  * ws: workspace of ctn_attn_fwd_ws_floats / ctn_attn_bwd_ws_floats floats (16-byte aligned, contents irrelevant before and
  * after, one per call that may run concurrently); -1 from these means arguments that the call would refuse.
  * Results do not depend on the order of blocks: the same bits on every run. */
@@ -285,6 +288,7 @@ typedef struct {
     const void* k; int64_t k_b, k_t, k_h;
     const void* v; int64_t v_b, v_t, v_h;
     void* o; int64_t o_b, o_t, o_h;
+    void* o_low;
     float* lse;
     const void* d_o; int64_t do_b, do_t, do_h;
     void* dq; int64_t dq_b, dq_t, dq_h;

@@ -165,7 +165,7 @@ class AttnArgs(C.Structure):
         ("k", _p), ("k_b", _i64), ("k_t", _i64), ("k_h", _i64),
         ("v", _p), ("v_b", _i64), ("v_t", _i64), ("v_h", _i64),
         ("o", _p), ("o_b", _i64), ("o_t", _i64), ("o_h", _i64),
-        ("lse", _p),
+        ("o_low", _p), ("lse", _p),
         ("d_o", _p), ("do_b", _i64), ("do_t", _i64), ("do_h", _i64),
         ("dq", _p), ("dq_b", _i64), ("dq_t", _i64), ("dq_h", _i64),
         ("dk", _p), ("dk_b", _i64), ("dk_t", _i64), ("dk_h", _i64),

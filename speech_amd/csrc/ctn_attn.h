@@ -115,11 +115,11 @@ template <typename T, int DT, int ROWS, int NT> struct Tile {
     u32x4 c[N][QUADS];
     int off[N];
     int pitch;                                                   // bytes
-    __device__ __forceinline__ void init(const int64_t stride, const int D) {
+    __device__ __forceinline__ void init(const int64_t stride, const int D, const int tid) {      // tid: index among the NT threads
         pitch = (int)stride * ES;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int q = threadIdx.x + NT * i, r = q / CPR, d = (q % CPR) * 8;
+            const int q = tid + NT * i, r = q / CPR, d = (q % CPR) * 8;
             off[i] = (WHOLE || r < ROWS) && d < D ? r * pitch + d * ES : 0x7fffff00;
         }
     }
@@ -132,10 +132,10 @@ template <typename T, int DT, int ROWS, int NT> struct Tile {
 #pragma unroll
             for (int h = 0; h < QUADS; ++h) c[i][h] = __builtin_amdgcn_raw_buffer_load_b128(r, off[i] + 16 * h, 0, 0);
     }
-    __device__ __forceinline__ void store(unsigned char* lds) const {
+    __device__ __forceinline__ void store(unsigned char* lds, const int tid) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int q = threadIdx.x + NT * i, r = q / CPR, ch = q % CPR;
+            const int q = tid + NT * i, r = q / CPR, ch = q % CPR;
             Frag<Planes<T>::N> f;
             if constexpr (ES == 2) {
                 f.p[0] = __builtin_bit_cast(bf16x8, c[i][0]);
@@ -199,6 +199,18 @@ __device__ __forceinline__ void store4(__bf16* p, const f32x4 v) {
     union { unsigned long long u; bf16x2 h[2]; } x;
     x.h[0] = __builtin_convertvector(f32x2{v[0], v[1]}, bf16x2), x.h[1] = __builtin_convertvector(f32x2{v[2], v[3]}, bf16x2);
     *reinterpret_cast<unsigned long long*>(p) = x.u;
+}
+
+// an output row's elements, and what their rounding left over
+__device__ __forceinline__ void store_out(float* p, void*, const int64_t, const f32x4 v) { ctn_st4(p, v); }
+__device__ __forceinline__ void store_out(__bf16* base, void* low, const int64_t at, const f32x4 v) {
+    store4(base, v);
+    if (low != nullptr) {
+        f32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = v[i] - (float)(__bf16)v[i];
+        store4((__bf16*)low + at, r);
+    }
 }
 
 // Block index -> (tile, unit), unit = a (batch element, head), `per` tiles each.  Blocks are dealt to the eight dies in turn;

@@ -7,7 +7,9 @@
 // score gradients leave the registers and every sum has one owner and a fixed order: the dQ kernel walks key tiles (and
 // forms delta on the way, for the second launch), the dK / dV kernel walks the query tiles of all query heads of its key
 // head.  Seven products where an order-free accumulation of dQ would need five: the price of the same bits on every run.
-// For bf16 tensors p and ds are rounded to bf16 (half a step, relative 2^-8 each at most) where they enter a product.
+// For bf16 tensors p and ds are rounded to bf16 (half a step, relative 2^-8 each at most) where they enter a product, which
+// adds about as much to a gradient as its own rounding does; in heads of up to 32 features, whose dq also feels what
+// the forward pass's roundings did to delta, dq takes ds in two pieces.
 #include "ctn_attn.h"
 
 bool ctn_attn_args_ok(const ctn_attn_args* a, const char* who);
@@ -60,16 +62,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int64_t kstep = KT * a.k_t, vstep = KT * a.v_t;
     int left = kend;
     tile_t tk, tv;
-    tk.init(a.k_t, a.D);
-    tv.init(a.v_t, a.D);
+    tk.init(a.k_t, a.D, threadIdx.x);
+    tv.init(a.v_t, a.D, threadIdx.x);
     auto fetch = [&]() {                                         // the next tile
         tk.load(kp, left, a.D);
         tv.load(vp, left, a.D);
         kp += kstep, vp += vstep, left -= KT;
     };
     auto stage = [&](const int buf) {
-        tk.store(lds + buf * BUF);
-        tv.store(lds + buf * BUF + tile_t::BYTES);
+        tk.store(lds + buf * BUF, threadIdx.x);
+        tv.store(lds + buf * BUF + tile_t::BYTES, threadIdx.x);
     };
     if (t1 > 0) fetch();
 
@@ -78,20 +80,36 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     {
         const T* qp = (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
         const T* gp = (const T*)a.d_o + b * a.do_b + tq * a.do_t + head * a.do_h;
-        const T* op = (const T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h;
+        const int64_t at = b * a.o_b + tq * a.o_t + head * a.o_h;
+        Chunk<T> cq[KS], cg[KS], co[KS], cl[NP == 1 ? KS : 1];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = 16 * s + 8 * half;
-            Chunk<T> cq, cg, co;
-            if (live && d < a.D) cq.load(qp + d), cg.load(gp + d), co.load(op + d);
-            else cq.zero(), cg.zero(), co.zero();
-            cq.frag(q[s]);
-            cg.frag(g[s]);
+            if (live && d < a.D) cq[s].load(qp + d), cg[s].load(gp + d), co[s].load((const T*)a.o + at + d);
+            else cq[s].zero(), cg[s].zero(), co[s].zero();
+        }
+        if constexpr (NP == 1) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = 16 * s + 8 * half;
+                if (a.o_low != nullptr && live && d < a.D) cl[s].load((const T*)a.o_low + at + d);
+                else cl[s].zero();
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            cq[s].frag(q[s]);
+            cg[s].frag(g[s]);
             float x[8], y[8];
-            cg.floats(x);
-            co.floats(y);
+            cg[s].floats(x);
+            co[s].floats(y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
+            if constexpr (NP == 1) {
+                cl[s].floats(y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
+            }
         }
     }
     delta = half_sum(delta);
@@ -137,12 +155,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = s[8 * i + e];
-                Frag<NP> ds;
+                Frag<NP> ds, low;
                 make_frag(x, ds);
+                if constexpr (NP == 1 && DT == 32) {             // narrow heads: what the rounding left over as well
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] -= (float)ds.p[0][e];
+                    make_frag(x, low);
+                }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<NP> k;
                     frag_cols<NP, DT, KT>(K, r0 + 16 * i, 32 * d, k);
+                    if constexpr (NP == 1 && DT == 32) mma(dq[d], k, low);
                     mma(dq[d], k, ds);
                 }
             }
@@ -202,8 +226,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
     }
 
     tile_t tq, tg;
-    tq.init(a.q_t, a.D);
-    tg.init(a.do_t, a.D);
+    tq.init(a.q_t, a.D, threadIdx.x);
+    tg.init(a.do_t, a.D, threadIdx.x);
     constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
     float stat[NS];
     auto fetch = [&](const int i) {
@@ -224,8 +248,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
     };
     auto stage = [&](const int buf) {
         unsigned char* p = lds + buf * BUF;
-        tq.store(p);
-        tg.store(p + tile_t::BYTES);
+        tq.store(p, threadIdx.x);
+        tg.store(p + tile_t::BYTES, threadIdx.x);
 #pragma unroll
         for (int x = 0; x < NS; ++x)
             if (threadIdx.x + NT * x < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[threadIdx.x + NT * x] = stat[x];

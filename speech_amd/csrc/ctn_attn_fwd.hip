@@ -6,8 +6,6 @@
 // row, and its probabilities are the B fragments of O^T += V^T P^T as they stand (ctn_attn.h).
 // Probabilities and output accumulate in fp32; for bf16 tensors the probabilities are rounded to bf16 for the second
 // product (relative 2^-8 each at most, averaged over the keys; their sum is taken before the rounding).
-// Few rows against many keys: the query heads of a key head become rows of one tile and the key range is split over blocks,
-// each leaving its normalised output and its log-sum to the caller's workspace; a second launch joins them.
 #include "ctn_attn.h"
 
 namespace {
@@ -21,7 +19,14 @@ struct fwd_params {
     float* po; float* pl;                 // split: partial outputs [nsplit][B H Tq][D] and log2-sums [nsplit][B H Tq]
 };
 
-template <typename T, int DT, int NW, int KT>
+// SHORT (bf16 training calls of up to 512 keys): rows that see at most FEW_KEYS keep what the probabilities' rounding drops, in
+// a second product.  Over many keys the roundings average out; over a few they are what the row sums d_o . o of the
+// backward pass, and with them the score gradients, are off by (causal sequences of 20 to 70 steps: gradients 1.6 times as far
+// from exact ones as their own rounding without it, 1.42 with it).  A variant of its own because the branch alone costs a
+// long sequence's loop a tenth.
+constexpr int FEW_KEYS = 128, SHORT_KEYS = 512;
+
+template <typename T, int DT, int NW, int KT, bool SHORT>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_fwd_kernel(const fwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, NK = KT / 32, ND = DT / 32;
     typedef Tile<T, DT, KT, NT> tile_t;
@@ -31,9 +36,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
     unsigned tile, unit;
-    deal(blockIdx.x, a.batch * f.heads, f.nqt * f.nsplit, a.causal, tile, unit);
-    const int sp = tile % f.nsplit;
-    const int qt = f.nqt - 1 - (int)(tile / f.nsplit);           // with a causal mask the last queries see the most keys
+    deal(blockIdx.x, a.batch * f.heads, f.nqt, a.causal, tile, unit);
+    const int qt = f.nqt - 1 - (int)tile;                        // with a causal mask the last queries see the most keys
     const int hh = unit % f.heads, b = unit / f.heads;
 
     const int w0 = (qt * NW + wave) * 32;                        // the wave's first row
@@ -54,25 +58,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     }
     if (w0 >= f.rows) wend = 0;
     const int ntile = kend > 0 ? (kend + KT - 1) / KT : 0;
-    const int t0 = (int)((int64_t)ntile * sp / f.nsplit), t1 = (int)((int64_t)ntile * (sp + 1) / f.nsplit);
 
-    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h + (int64_t)t0 * KT * a.k_t;
-    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h + (int64_t)t0 * KT * a.v_t;
+    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h;
+    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h;
     const int64_t kstep = KT * a.k_t, vstep = KT * a.v_t;
-    int left = kend - t0 * KT;
+    int left = kend;
     tile_t tk, tv;
-    tk.init(a.k_t, a.D);
-    tv.init(a.v_t, a.D);
+    tk.init(a.k_t, a.D, threadIdx.x);
+    tv.init(a.v_t, a.D, threadIdx.x);
     auto fetch = [&]() {                                         // the next tile
         tk.load(kp, left, a.D);
         tv.load(vp, left, a.D);
         kp += kstep, vp += vstep, left -= KT;
     };
     auto stage = [&](const int buf) {
-        tk.store(lds + buf * BUF);
-        tv.store(lds + buf * BUF + tile_t::BYTES);
+        tk.store(lds + buf * BUF, threadIdx.x);
+        tv.store(lds + buf * BUF + tile_t::BYTES, threadIdx.x);
     };
-    if (t0 < t1) fetch();
+    if (ntile > 0) fetch();
 
     Frag<NP> q[KS];
     {
@@ -93,12 +96,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    if (t0 < t1) stage(0);
+    if (ntile > 0) stage(0);
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const unsigned char* K = lds + ((t - t0) & 1) * BUF;
+    for (int t = 0; t < ntile; ++t) {
+        const unsigned char* K = lds + (t & 1) * BUF;
         const unsigned char* V = K + tile_t::BYTES;
-        if (t + 1 < t1) fetch();
+        if (t + 1 < ntile) fetch();
         if (t * KT < wend) {
             f32x16 s[NK];
 #pragma unroll
@@ -152,9 +155,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
                     frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
                     mma(o[d], v, p);
                 }
+                if (SHORT && wend <= FEW_KEYS) {                 // what the rounding left over
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] -= (float)p.p[0][e];
+                    make_frag(x, p);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        Frag<NP> v;
+                        frag_cols<NP, DT, KT>(V, 16 * i, 32 * d, v);
+                        mma(o[d], v, p);
+                    }
+                }
             }
         }
-        if (t + 1 < t1) stage((t - t0 + 1) & 1);
+        if (t + 1 < ntile) stage((t + 1) & 1);
         __syncthreads();
     }
 
@@ -162,53 +176,229 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     if (!live) return;
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const float lse = l > 0.f ? m * f.sl2 + __builtin_amdgcn_logf(l) : -INFINITY;
-    const int64_t row = ((int64_t)b * a.H + head) * a.Tq + tq, nrow = (int64_t)a.batch * a.H * a.Tq;
-    float* po = f.po + (sp * nrow + row) * a.D;
-    T* op = (T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h;
+    const int64_t at = b * a.o_b + tq * a.o_t + head * a.o_h;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int c = 32 * d + acc_row(e);
-            const f32x4 v = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv;
-            if (c < a.D) {
-                if (f.nsplit > 1) ctn_st4(po + c, v);
-                else store4(op + c, v);
+            if (c < a.D) store_out((T*)a.o + at + c, a.o_low, at + c, f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv);
+        }
+    if (half == 0 && a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + tq] = lse;
+}
+
+// ------------------------------------------------------------------------------------------------ few rows, many keys
+// At most 32 rows (the queries of every head of a key head) against a long run of keys: single tokens against a cache.  Bound
+// by reading the keys and values once; every wave of a block walks its own 32-key tiles (tile w of the block's range, w + W,
+// ...) without a barrier: the keys go straight from memory into A fragments (lane = key; eight consecutive features per
+// load), the values through LDS of the wave's own for the transposing read, the next tile of both in flight during the
+// current one's products.  The waves' results meet in LDS in the waves' order; where the keys are split over blocks the joined
+// results go to the caller's workspace and a second launch joins those.
+template <typename T, int DT> constexpr int few_waves() { return Planes<T>::N * DT > 192 ? 4 : 8; }
+
+template <typename T, int DT>
+__global__ __launch_bounds__((few_waves<T, DT>() * 64)) void attn_few_kernel(const fwd_params f) {
+    constexpr int NP = Planes<T>::N, W = few_waves<T, DT>(), KS = DT / 16, ND = DT / 32;
+    typedef Tile<T, DT, 32, 64> tile_t;                          // of one wave
+    constexpr int OWN = tile_t::BYTES > 32 * DT * 4 ? tile_t::BYTES : 32 * DT * 4;       // values, later the wave's output
+    __shared__ __attribute__((aligned(16))) unsigned char lds[W * OWN + W * 32 * 8];
+    float* const ml = reinterpret_cast<float*>(lds + W * OWN);   // [W][32] maxima, [W][32] sums
+    const ctn_attn_args& a = f.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
+    const int off = a.Tk - a.Tq;
+    const int sp = blockIdx.x % f.nsplit;
+    const unsigned unit = blockIdx.x / f.nsplit;
+    const int hk = unit % f.heads, b = unit / f.heads;
+    const bool live = l31 < f.rows;
+    const int g = l31 / a.Tq, tq = l31 - g * a.Tq, head = hk * f.G + g;
+    int len = a.Tk;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
+    const int vis = !live ? 0 : a.causal ? min(len, tq + off + 1) : len;
+    const int kend = a.causal ? min(len, a.Tq + off) : len, wfull = a.causal ? min(len, off + 1) : len;
+    const int ntile = kend > 0 ? (kend + 31) / 32 : 0;
+    const int t0 = (int)((int64_t)ntile * sp / f.nsplit), t1 = (int)((int64_t)ntile * (sp + 1) / f.nsplit);
+
+    unsigned char* const own = lds + wave * OWN;
+    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h + (int64_t)(t0 + wave) * 32 * a.k_t;
+    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h + (int64_t)(t0 + wave) * 32 * a.v_t;
+    const int64_t kstep = 32 * W * a.k_t, vstep = 32 * W * a.v_t;
+    const int kpitch = (int)a.k_t * (int)sizeof(T);
+    int koff[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) koff[s] = 16 * s + 8 * half < a.D ? l31 * kpitch + (16 * s + 8 * half) * (int)sizeof(T) : 0x7fffff00;
+    int left = kend - (t0 + wave) * 32;
+    tile_t tv;
+    tv.init(a.v_t, a.D, lane);
+    u32x4 kr[KS][tile_t::QUADS];
+    auto fetch = [&]() {
+        const int rows = left < 32 ? left : 32;
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, rows > 0 ? (rows - 1) * kpitch + a.D * (int)sizeof(T) : 0, 0x00020000);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int h = 0; h < tile_t::QUADS; ++h) kr[s][h] = __builtin_amdgcn_raw_buffer_load_b128(rs, koff[s] + 16 * h, 0, 0);
+        tv.load(vp, left, a.D);
+        kp += kstep, vp += vstep, left -= 32 * W;
+    };
+    int t = t0 + wave;
+    if (t < t1) fetch();
+
+    Frag<NP> q[KS];
+    {
+        const T* qp = (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            Chunk<T> c;
+            const int d = 16 * s + 8 * half;
+            if (live && d < a.D) c.load(qp + d);
+            else c.zero();
+            c.frag(q[s]);
+        }
+    }
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (; t < t1; t += W) {
+        f32x16 s;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            Frag<NP> k;
+            if constexpr (NP == 1) {
+                k.p[0] = __builtin_bit_cast(bf16x8, kr[i][0]);
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(kr[i][tile_t::QUADS == 2 ? e >> 2 : 0][e & 3]);
+                make_frag(x, k);
+            }
+            mma(s, k, q[i]);
+        }
+        tv.store(own, lane);                                // a wave's LDS accesses run in order: no wait for the last tile's reads
+        if (t + W < t1) fetch();
+        if ((t + 1) * 32 > wfull) {
+            const int lim = vis - t * 32 - 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = (e & 3) + 8 * (e >> 2) < lim ? s[e] : -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
+        const float mn = fmaxf(m, half_max(mx));
+        const float base = mn == -INFINITY ? 0.f : mn * f.sl2;
+        if (__any(mn != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m * f.sl2 - base);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        }
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * i + e], f.sl2, -base));
+                l += x[e];
+            }
+            Frag<NP> p;
+            make_frag(x, p);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                Frag<NP> v;
+                frag_cols<NP, DT, 32>(own, 16 * i, 32 * d, v);
+                mma(o[d], v, p);
             }
         }
-    if (half == 0) {
-        if (f.nsplit > 1) f.pl[sp * nrow + row] = lse;
-        else if (a.lse) a.lse[row] = lse;
+    }
+    l = half_sum(l);
+    __syncthreads();                                             // (reached by every wave: no return above)
+    float* const mine = reinterpret_cast<float*>(own);           // [row][feature], chunks of four turned by the row
+    if (live) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                ctn_st4(mine + l31 * DT + 4 * (((32 * d + acc_row(e)) >> 2) ^ (l31 & 7)),
+                        f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]});
+        if (half == 0) ml[wave * 32 + l31] = m, ml[(W + wave) * 32 + l31] = l;
+    }
+    __syncthreads();
+    const int64_t nrow = (int64_t)a.batch * a.H * a.Tq;
+    for (int i = threadIdx.x; i < f.rows * (DT / 4); i += W * 64) {
+        const int r = i / (DT / 4), ch = i % (DT / 4);
+        if (4 * ch >= a.D) continue;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, ml[w * 32 + r]);
+        const float base = mx == -INFINITY ? 0.f : mx * f.sl2;
+        float tot = 0.f;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float c = __builtin_amdgcn_exp2f(ml[w * 32 + r] * f.sl2 - base);
+            tot += c * ml[(W + w) * 32 + r];
+            x += ctn_ld4(reinterpret_cast<const float*>(lds + w * OWN) + r * DT + 4 * (ch ^ (r & 7))) * c;
+        }
+        const float inv = tot > 0.f ? 1.f / tot : 0.f;
+        const float lse = tot > 0.f ? base + __builtin_amdgcn_logf(tot) : -INFINITY;
+        const int gr = r / a.Tq, tr = r - gr * a.Tq, hr = hk * f.G + gr;
+        const int64_t row = ((int64_t)b * a.H + hr) * a.Tq + tr;
+        if (f.nsplit > 1) {
+            ctn_st4(f.po + (sp * nrow + row) * a.D + 4 * ch, x * inv);
+            if (ch == 0) f.pl[sp * nrow + row] = lse;
+        } else {
+            const int64_t at = b * a.o_b + tr * a.o_t + hr * a.o_h + 4 * ch;
+            store_out((T*)a.o + at, a.o_low, at, x * inv);
+            if (ch == 0 && a.lse) a.lse[row] = lse;
+        }
     }
 }
 
-// Joins the key ranges of a row: o = sum_s 2^(l_s - max) o_s / sum_s 2^(l_s - max).  One wave per row, lanes along D.
+// Joins the key ranges of a row: o = sum_s 2^(l_s - max) o_s / sum_s 2^(l_s - max).  A block per row: 32 threads along the
+// features, four at a time, eight ranges side by side.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const fwd_params f) {
+    __shared__ float part[8][128 + 4];
+    __shared__ float tots[8];
     const ctn_attn_args& a = f.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t nrow = (int64_t)a.batch * a.H * a.Tq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= nrow) return;
+    const int c = (threadIdx.x & 31) * 4, p = threadIdx.x >> 5;
+    const int64_t nrow = (int64_t)a.batch * a.H * a.Tq, row = blockIdx.x;
     const int tq = row % a.Tq, head = row / a.Tq % a.H;
     const int64_t b = row / a.Tq / a.H;
     float mx = -INFINITY;
-    for (int s = 0; s < f.nsplit; ++s) mx = fmaxf(mx, f.pl[s * nrow + row]);
-    float tot = 0.f, x[2] = {0.f, 0.f};
-    if (mx != -INFINITY)
-        for (int s = 0; s < f.nsplit; ++s) {
-            const float ls = f.pl[s * nrow + row];
-            if (ls == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(ls - mx);
-            tot += w;
+#pragma unroll 4
+    for (int s = threadIdx.x & 31; s < f.nsplit; s += 32) mx = fmaxf(mx, f.pl[s * nrow + row]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (lane + 64 * i < a.D) x[i] += w * f.po[(s * nrow + row) * a.D + lane + 64 * i];
-        }
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float tot = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = p; s < f.nsplit; s += 8) {
+        const float w = __builtin_amdgcn_exp2f(f.pl[s * nrow + row] - base);
+        tot += w;
+        if (c < a.D) x += ctn_ld4(f.po + (s * nrow + row) * a.D + c) * w;
+    }
+    if (c < a.D) ctn_st4(&part[p][c], x);
+    if ((threadIdx.x & 31) == 0) tots[p] = tot;
+    __syncthreads();
+    if (p != 0) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+        tot += tots[w];
+        if (c < a.D) x += ctn_ld4(&part[w][c]);
+    }
     const float inv = tot > 0.f ? 1.f / tot : 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < a.D) ((T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h)[lane + 64 * i] = (T)(x[i] * inv);
-    if (a.lse && lane == 0) a.lse[row] = tot > 0.f ? mx + __builtin_amdgcn_logf(tot) : -INFINITY;
+    const int64_t at = b * a.o_b + tq * a.o_t + head * a.o_h + c;
+    if (c < a.D) store_out((T*)a.o + at, a.o_low, at, x * inv);
+    if (a.lse && threadIdx.x == 0) a.lse[row] = tot > 0.f ? base + __builtin_amdgcn_logf(tot) : -INFINITY;
 }
 
 // Keys per tile: 64, halved where the LDS of three planes would keep a third block off the CU (fp32 heads of 64 features,
@@ -218,31 +408,37 @@ template <typename T, int DT, int NW> constexpr int key_tile() {
 }
 
 // How the call is cut.  Packed: all query heads of a key head in one tile of at most 128 rows, where there are fewer than
-// 32 queries (a tile per head would leave most of its 32 rows empty and read the keys once per query head).
-struct fwd_cut { bool packed; int rows, nw, nqt, heads, nsplit; };
+// 32 queries (a tile per head would leave most of its 32 rows empty and read the keys once per query head).  Few: at
+// most 32 such rows against 128 keys or more take the kernel above, its keys split over blocks until there is one a CU (40000
+// keys of 8 heads of 128 features, bf16: 33 us; two a CU 41 us) -- two where lengths make the sequences unequal (8 sequences
+// of up to 32768 keys: 130 us against 146 us) -- but into no less than two tiles a wave.
+struct fwd_cut { bool packed, few; int rows, nw, nqt, heads, nsplit; };
 fwd_cut cut_forward(const ctn_attn_args& a) {
     fwd_cut c;
     const int G = a.H / a.Hk;
-    c.packed = G > 1 && a.Tq < 32 && (int64_t)G * a.Tq <= 128;
+    c.packed = a.Tq < 32 && (int64_t)G * a.Tq <= 128;
     c.rows = c.packed ? G * a.Tq : a.Tq;
     c.heads = c.packed ? a.Hk : a.H;
+    c.few = c.packed && c.rows <= 32 && a.Tk >= 128;
     c.nw = c.rows <= 32 ? 1 : c.rows <= 64 ? 2 : 4;
     c.nqt = ctn_cdiv(c.rows, 32 * c.nw);
     c.nsplit = 1;
-    const int64_t blocks = (int64_t)a.batch * c.heads * c.nqt;
-    const int tiles = ctn_cdiv(a.Tk, 64);
-    if (c.nqt == 1 && blocks < 512) {
-        // split the keys until there are about eight waves for every CU, at least four tiles a piece
-        int64_t n = 2048 / (blocks * c.nw);
-        if (n > tiles / 4) n = tiles / 4;
-        if (n > 1) c.nsplit = (int)n;
+    if (c.few) {
+        const int64_t units = (int64_t)a.batch * a.Hk;
+        int64_t n = (a.lengths ? 512 : 256) / units, most = a.Tk / (32 * 8 * 2);
+        if (n > most) n = most;
+        c.nsplit = n < 1 ? 1 : (int)n;
     }
     return c;
 }
 
 template <typename T, int DT, int NW>
 void launch_fwd(const fwd_params& f, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, key_tile<T, DT, NW>()>), dim3(grid), dim3(NW * 64), 0, s, f);
+    constexpr int KT = key_tile<T, DT, NW>();
+    if (Planes<T>::N == 1 && f.a.o_low != nullptr && f.a.Tk <= SHORT_KEYS)
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, KT, Planes<T>::N == 1>), dim3(grid), dim3(NW * 64), 0, s, f);
+    else
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DT, NW, KT, false>), dim3(grid), dim3(NW * 64), 0, s, f);
 }
 template <typename T, int DT>
 void launch_fwd_nw(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
@@ -250,8 +446,18 @@ void launch_fwd_nw(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
     else if (nw == 2) launch_fwd<T, DT, 2>(f, grid, s);
     else launch_fwd<T, DT, 4>(f, grid, s);
 }
+template <typename T, int DT>
+void launch_few(const fwd_params& f, unsigned grid, hipStream_t s) {
+    hipLaunchKernelGGL((attn_few_kernel<T, DT>), dim3(grid), dim3(few_waves<T, DT>() * 64), 0, s, f);
+}
 template <typename T>
-void launch_fwd_type(const fwd_params& f, int nw, unsigned grid, hipStream_t s) {
+void launch_fwd_type(const fwd_params& f, int nw, bool few, unsigned grid, hipStream_t s) {
+    if (few) {
+        if (f.a.D <= 32) launch_few<T, 32>(f, grid, s);
+        else if (f.a.D <= 64) launch_few<T, 64>(f, grid, s);
+        else launch_few<T, 128>(f, grid, s);
+        return;
+    }
     if (f.a.D <= 32) launch_fwd_nw<T, 32>(f, nw, grid, s);
     else if (f.a.D <= 64) launch_fwd_nw<T, 64>(f, nw, grid, s);
     else launch_fwd_nw<T, 128>(f, nw, grid, s);
@@ -309,13 +515,13 @@ int ctn_attn_fwd(const ctn_attn_args* a, void* stream) {
         f.po = a->ws, f.pl = a->ws + c.nsplit * nrow * a->D;
     }
     const int64_t grid = (int64_t)a->batch * c.heads * c.nqt * c.nsplit;
-    CTN_REQUIRE(grid < 0x7fffffff && (nrow + 3) / 4 < 0x7fffffff, "ctn_attn_fwd: too much work for one launch");
+    CTN_REQUIRE(grid < 0x7fffffff && (c.nsplit == 1 || nrow < 0x7fffffff), "ctn_attn_fwd: too much work for one launch");
     hipStream_t s = (hipStream_t)stream;
-    if (a->type == CTN_TYPE_F32) launch_fwd_type<float>(f, c.nw, (unsigned)grid, s);
-    else launch_fwd_type<__bf16>(f, c.nw, (unsigned)grid, s);
+    if (a->type == CTN_TYPE_F32) launch_fwd_type<float>(f, c.nw, c.few, (unsigned)grid, s);
+    else launch_fwd_type<__bf16>(f, c.nw, c.few, (unsigned)grid, s);
     CTN_CHECK_LAUNCH("ctn_attn_fwd");
     if (c.nsplit > 1) {
-        const dim3 jg((unsigned)((nrow + 3) / 4));
+        const dim3 jg((unsigned)nrow);
         if (a->type == CTN_TYPE_F32) hipLaunchKernelGGL(attn_join_kernel<float>, jg, dim3(256), 0, s, f);
         else hipLaunchKernelGGL(attn_join_kernel<__bf16>, jg, dim3(256), 0, s, f);
         CTN_CHECK_LAUNCH("ctn_attn_fwd (join)");

@@ -632,17 +632,17 @@ class AttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, causal, scale):
-        o, lse = ops.attn_fwd(q, k, v, lengths, causal, scale)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        o, lse, low = ops.attn_fwd(q, k, v, lengths, causal, scale)
+        ctx.save_for_backward(q, k, v, o, lse, low, lengths)
         ctx.meta = (causal, scale)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, lse, low, lengths = ctx.saved_tensors
         causal, scale = ctx.meta
-        dq, dk, dv = ops.attn_bwd(do, q, k, v, o, lse, lengths, causal, scale, ctx.needs_input_grad[:3])
+        dq, dk, dv = ops.attn_bwd(do, q, k, v, o, lse, low, lengths, causal, scale, ctx.needs_input_grad[:3])
         return dq, dk, dv, None, None, None
 
 

@@ -510,7 +510,7 @@ def _attn_operand(x, shape):
 
 
 # the fields of ctn_attn_args in their order
-_ATTN_PACK = struct.Struct("8if i" + "Q" + "Qqqq" * 4 + "Q" + "Qqqq" * 4 + "Qq").pack
+_ATTN_PACK = struct.Struct("8if i" + "Q" + "Qqqq" * 4 + "QQ" + "Qqqq" * 4 + "Qq").pack
 _ATTN_NONE = (0, 0, 0, 0)
 
 
@@ -536,10 +536,10 @@ def check_attention(q, k, v, lengths):
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_ws(B, Tq, Tk, H, Hk, D, code, backward):
+def _attn_ws(B, Tq, Tk, H, Hk, D, code, ragged, backward):
     """Workspace floats of a call of these sizes."""
     a = _lib.AttnArgs(batch=B, Tq=Tq, Tk=Tk, H=H, Hk=Hk, D=D, type=code, scale=1.0, q=16, k=16, v=16, o=16, q_t=D, k_t=D, v_t=D,
-                      o_t=D)
+                      o_t=D, lengths=16 if ragged else None)
     lib = _lib.load()
     need = (lib.ctn_attn_bwd_ws_floats if backward else lib.ctn_attn_fwd_ws_floats)(C.byref(a))
     if need < 0:
@@ -556,7 +556,8 @@ def _attn_lengths(lengths, Tk):
 
 
 def attn_fwd(q, k, v, lengths=None, causal=False, scale=None, want_lse=True):
-    """q (B, Tq, H, D), k, v (B, Tk, Hk, D) -> o dense like q, lse (B, H, Tq) fp32 (None unless wanted); see ctn_attn_fwd."""
+    """q (B, Tq, H, D), k, v (B, Tk, Hk, D) -> o dense like q, and for attn_bwd (None unless wanted) lse (B, H, Tq) fp32 and, for
+    bf16 tensors, o's rounding errors; see ctn_attn_fwd."""
     lib = _lib.load()
     code = check_attention(q, k, v, lengths)
     B, Tq, H, D = qs = q.shape
@@ -567,17 +568,18 @@ def attn_fwd(q, k, v, lengths=None, causal=False, scale=None, want_lse=True):
     lengths = _attn_lengths(lengths, Tk)
     o = q.new_empty(qs)
     lse = q.new_empty((B, H, Tq), dtype=torch.float32) if want_lse else None
-    need = _attn_ws(B, Tq, Tk, H, Hk, D, code, False)
+    low = q.new_empty(qs) if want_lse and code == _lib.TYPE_BF16 else None
+    need = _attn_ws(B, Tq, Tk, H, Hk, D, code, lengths is not None, False)
     ws = q.new_empty((need,), dtype=torch.float32) if need else None
     args = _lib.AttnArgs.from_buffer_copy(_ATTN_PACK(
         B, Tq, Tk, H, Hk, D, code, 1 if causal else 0, D ** -0.5 if scale is None else scale, 0, _ptr(lengths) or 0,
         q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, o.data_ptr(), Tq * H * D, H * D, D,
-        _ptr(lse) or 0, *_ATTN_NONE, *_ATTN_NONE, *_ATTN_NONE, *_ATTN_NONE, _ptr(ws) or 0, need))
+        _ptr(low) or 0, _ptr(lse) or 0, *_ATTN_NONE, *_ATTN_NONE, *_ATTN_NONE, *_ATTN_NONE, _ptr(ws) or 0, need))
     _enqueue("ctn_attn_fwd", q.get_device(), lib.ctn_attn_fwd, args)
-    return o, lse
+    return o, lse, low
 
 
-def attn_bwd(do, q, k, v, o, lse, lengths=None, causal=False, scale=None, want=(True, True, True)):
+def attn_bwd(do, q, k, v, o, lse, low, lengths=None, causal=False, scale=None, want=(True, True, True)):
     """-> dq, dk, dv (dense, each None unless wanted) from the gradient of o and what attn_fwd returned; see ctn_attn_bwd."""
     lib = _lib.load()
     code = check_attention(q, k, v, lengths)
@@ -592,13 +594,13 @@ def attn_bwd(do, q, k, v, o, lse, lengths=None, causal=False, scale=None, want=(
     dq = q.new_empty(qs) if want[0] else None
     dk = q.new_empty(ks) if want[1] else None
     dv = q.new_empty(ks) if want[2] else None
-    need = _attn_ws(B, Tq, Tk, H, Hk, D, code, True)
+    need = _attn_ws(B, Tq, Tk, H, Hk, D, code, lengths is not None, True)
     ws = q.new_empty((need,), dtype=torch.float32) if need else None
     dense_k = (Tk * Hk * D, Hk * D, D)
     args = _lib.AttnArgs.from_buffer_copy(_ATTN_PACK(
         B, Tq, Tk, H, Hk, D, code, 1 if causal else 0, D ** -0.5 if scale is None else scale, 0, _ptr(lengths) or 0,
         q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, o.data_ptr(), Tq * H * D, H * D, D,
-        lse.data_ptr(), do.data_ptr(), gb, gt, gh, _ptr(dq) or 0, Tq * H * D, H * D, D, _ptr(dk) or 0, *dense_k,
+        _ptr(low) or 0, lse.data_ptr(), do.data_ptr(), gb, gt, gh, _ptr(dq) or 0, Tq * H * D, H * D, D, _ptr(dk) or 0, *dense_k,
         _ptr(dv) or 0, *dense_k, _ptr(ws) or 0, need))
     _enqueue("ctn_attn_bwd", q.get_device(), lib.ctn_attn_bwd, args)
     return dq, dk, dv

@@ -195,8 +195,8 @@ def test_dual_path_attention_model_config_and_keys(tmp_path):
 
 def test_attention_workspace_of_every_size_the_wrapper_asks_for():
     for code in (_lib.TYPE_F32, _lib.TYPE_BF16):
-        assert ops._attn_ws(2, 3, 3, 2, 1, 16, code, True) >= 2 * 2 * 3
-        assert ops._attn_ws(2, 300, 300, 2, 1, 16, code, False) == 0
-        assert ops._attn_ws(1, 1, 100000, 2, 1, 16, code, False) > 0
+        assert ops._attn_ws(2, 3, 3, 2, 1, 16, code, False, True) >= 2 * 2 * 3
+        assert ops._attn_ws(2, 300, 300, 2, 1, 16, code, True, False) == 0
+        assert ops._attn_ws(1, 1, 100000, 2, 1, 16, code, False, False) > 0
     with pytest.raises(_lib.CtnError):
-        ops._attn_ws(2, 3, 3, 2, 1, 12, _lib.TYPE_F32, True)
+        ops._attn_ws(2, 3, 3, 2, 1, 12, _lib.TYPE_F32, False, True)
