@@ -178,7 +178,20 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_fwd_kernel(const T* 
     }
 }
 
-// part: [gridDim.x][2][C] column sums of dy xhat and dy over the block's rows; null: not formed
+// a column's two sums to their place: the block's part of the workspace, or (part null) the parameters' gradients themselves
+__device__ __forceinline__ void fcolumn(float* part, void* dgamma, void* dbeta, const bool wbf, const int C, const int c, const int w,
+                                        const float t) {
+    if (part != nullptr) {
+        part[w * C + c] = t;
+        return;
+    }
+    void* out = w == 0 ? dgamma : dbeta;
+    if (out == nullptr) return;
+    if (wbf) ((__bf16*)out)[c] = (__bf16)t;
+    else ((float*)out)[c] = t;
+}
+
+// part: [gridDim.x][2][C] column sums of dy xhat and dy over the block's rows; null: one block, the sums go to dgamma and dbeta
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* __restrict__ dy, const int64_t lddy,
                                                                        const T* __restrict__ x, const int64_t ldx,
@@ -186,7 +199,7 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* 
                                                                        const void* __restrict__ gamma, const bool wbf,
                                                                        const float* __restrict__ stats,
                                                                        T* __restrict__ dx, const int64_t lddx,
-                                                                       float* __restrict__ part) {
+                                                                       float* __restrict__ part, void* dgamma, void* dbeta) {
     constexpr int V = FVec<T>::V, NT = fthreads<G>(), RPB = NT / G;
     constexpr int CW = G < 64 ? G : 64;                          // lanes of a wave that hold distinct columns
     __shared__ float red[2][2 * (G > 64 ? G / 64 : 1)];
@@ -254,8 +267,8 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* 
             }
         }
     }
-    if (part == nullptr) return;
-    float* out = part + (int64_t)blockIdx.x * 2 * C;
+    if (part == nullptr && dgamma == nullptr && dbeta == nullptr) return;
+    float* out = part == nullptr ? nullptr : part + (int64_t)blockIdx.x * 2 * C;
     if constexpr (G <= 64) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -274,7 +287,7 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* 
                 const int i = c % V, gg = (c / V) % G, k = c / (V * G);
                 float t = 0.f;
                 for (int q = 0; q < NT / 64; ++q) t += fold[(q * CW + gg) * NV * V + k * V + i];
-                out[w * C + c] = t;
+                fcolumn(out, dgamma, dbeta, wbf, C, c, w, t);
             }
             __syncthreads();
         }
@@ -284,7 +297,9 @@ __global__ __launch_bounds__(fthreads<G>()) void frame_norm_bwd_kernel(const T* 
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int c = (k * G + g) * V + i;
-                if (c < C) out[c] = dg[k][i], out[C + c] = db[k][i];
+                if (c >= C) continue;
+                fcolumn(out, dgamma, dbeta, wbf, C, c, 0, dg[k][i]);
+                fcolumn(out, dgamma, dbeta, wbf, C, c, 1, db[k][i]);
             }
     }
 }
@@ -320,9 +335,10 @@ int frame_rpb(const int C, const int V) {
     return n <= 8 ? 32 : n <= 16 ? 16 : n <= 32 ? 8 : n <= 128 ? 4 : 1;
 }
 // blocks of the backward pass: up to four of 256 threads a CU, at least 16 row groups each so that the column sums'
-// stores stay below a twentieth of the rows' own traffic
+// stores stay below a twentieth of the rows' own traffic; few rows in one block, which needs no second launch
 int frame_bwd_blocks(const int64_t R, const int C, const int V) {
     const int64_t groups = (R + frame_rpb(C, V) - 1) / frame_rpb(C, V);
+    if (groups <= 4) return 1;
     int64_t nb = (groups + 15) / 16;
     if (nb < 256) nb = groups < 256 ? groups : 256;
     return (int)(nb > 1024 ? 1024 : nb);
@@ -374,7 +390,8 @@ int ctn_frame_norm_fwd(const void* x, int64_t ldx, int64_t R, int C, int type, c
 
 int64_t ctn_frame_norm_bwd_ws_floats(int64_t R, int C, int type) {
     if (!frame_type_ok(type) || R <= 0 || C <= 0 || C > FRAME_MAX_C) return 0;
-    return (int64_t)frame_bwd_blocks(R, C, type == CTN_TYPE_F32 ? 4 : 8) * 2 * C;
+    const int nb = frame_bwd_blocks(R, C, type == CTN_TYPE_F32 ? 4 : 8);
+    return nb > 1 ? (int64_t)nb * 2 * C : 0;
 }
 
 int ctn_frame_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t R, int C, int type,
@@ -387,20 +404,20 @@ int ctn_frame_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
     const bool params = dgamma != nullptr || dbeta != nullptr;
     const int V = type == CTN_TYPE_F32 ? 4 : 8;
     const int nb = R > 0 ? frame_bwd_blocks(R, C, V) : 0;
-    CTN_REQUIRE(!params || nb == 0 || (ws && ws_floats >= (int64_t)nb * 2 * C),
+    CTN_REQUIRE(!params || nb <= 1 || (ws && ws_floats >= (int64_t)nb * 2 * C),
                 "ctn_frame_norm_bwd: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)nb * 2 * C);
     const bool wbf = wtype == CTN_TYPE_BF16;
-    float* part = params ? ws : nullptr;
+    float* part = params && nb > 1 ? ws : nullptr;
     if (nb > 0) {
 #define FRAME_BWD(T, G, NV)                                                                                                    \
     hipLaunchKernelGGL((frame_norm_bwd_kernel<T, G, NV>), dim3(nb), dim3(fthreads<G>()), 0, (hipStream_t)stream, (const T*)dy, \
-                       lddy, (const T*)x, ldx, R, C, gamma, wbf, stats, (T*)dx, lddx, part)
+                       lddy, (const T*)x, ldx, R, C, gamma, wbf, stats, (T*)dx, lddx, part, dgamma, dbeta)
         if (type == CTN_TYPE_F32) FRAME_DISPATCH(float, FRAME_BWD);
         else FRAME_DISPATCH(__bf16, FRAME_BWD);
 #undef FRAME_BWD
         CTN_CHECK_LAUNCH("ctn_frame_norm_bwd");
     }
-    if (params) {
+    if (params && nb != 1) {                              // (no rows: the sums of none)
         hipLaunchKernelGGL(frame_norm_param_kernel, dim3(ctn_cdiv(2 * (int64_t)C, 64)), dim3(1024), 0, (hipStream_t)stream, part, nb, C,
                            dgamma, dbeta, wbf);
         CTN_CHECK_LAUNCH("ctn_frame_norm_bwd (parameters)");

@@ -589,6 +589,16 @@ class LstmFn(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------------------------------------ frame norm, rotary positions, attention
+def _differentiated_once(backward):
+    """A backward pass whose results cannot be differentiated again.  once_differentiable costs about as much host time as the
+    launches of a short sequence, and has nothing to do unless the caller builds a graph of the backward pass."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(run)
+
+
 class FrameNormFn(torch.autograd.Function):
     """Layer norm over the last axis of x (..., C), parameters (C,) in fp32 or x's type (None: not applied)."""
 
@@ -599,8 +609,7 @@ class FrameNormFn(torch.autograd.Function):
         ctx.beta_dtype = None if beta is None else beta.dtype
         return y if x.dim() == 2 else y.view(x.shape)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiated_once
     def backward(ctx, dy):
         x, gamma, stats = ctx.saved_tensors
         need_x, need_g, need_b, _ = ctx.needs_input_grad
@@ -618,8 +627,7 @@ class RotaryFn(torch.autograd.Function):
         ctx.save_for_backward(turns, positions)
         return ops.rotary(x, turns, positions, first, interleaved, False, magnitude)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiated_once
     def backward(ctx, dy):
         turns, positions = ctx.saved_tensors
         first, interleaved, magnitude = ctx.meta
@@ -637,8 +645,7 @@ class AttentionFn(torch.autograd.Function):
         ctx.meta = (causal, scale)
         return o
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiated_once
     def backward(ctx, do):
         q, k, v, o, lse, low, lengths = ctx.saved_tensors
         causal, scale = ctx.meta

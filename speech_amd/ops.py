@@ -406,54 +406,56 @@ def _frame_norm_ws(R, Cc, code):
     return _lib.load().ctn_frame_norm_bwd_ws_floats(R, Cc, code)
 
 
-def _frame_norm_param_type(x2, gamma, beta):
-    """CTN_TYPE_* of the parameters, which are checked."""
-    code = _type(x2, "frame_norm")
-    if gamma is None and beta is None:
-        return code, code
-    _same_place("frame_norm", x2, gamma, beta)
-    dt = None
+def _frame_norm_types(x2, gamma, beta):
+    """CTN_TYPE_* of the rows and of the parameters, which are checked."""
+    code = _TYPES.get(x2.dtype)
+    if code is None or not x2.is_cuda:
+        _require_cuda(x2)
+        _type(x2, "frame_norm")
+    Cc, wdtype = x2.shape[1], None
     for w in (gamma, beta):
         if w is None:
             continue
-        if w.numel() != x2.shape[1] or not w.is_contiguous():
-            raise _lib.CtnError("frame_norm: parameters of {} contiguous elements, got {}".format(x2.shape[1], tuple(w.shape)))
-        if w.dtype != torch.float32 and w.dtype != x2.dtype or dt is not None and w.dtype != dt:
-            raise _lib.CtnError("frame_norm: parameters in float32 or the input's type, both alike")
+        if w.shape != (Cc,) or not w.is_contiguous():
+            raise _lib.CtnError("frame_norm: parameters of {} contiguous elements, got {}".format(Cc, tuple(w.shape)))
         dt = w.dtype
-    return code, _TYPES[dt]
+        if dt is not torch.float32 and dt is not x2.dtype or wdtype is not None and dt is not wdtype:
+            raise _lib.CtnError("frame_norm: parameters in float32 or the input's type, both alike")
+        if w.get_device() != x2.get_device():
+            _same_place("frame_norm", x2, w)
+        wdtype = dt
+    return code, code if wdtype is None else _TYPES[wdtype]
 
 
 def frame_norm_fwd(x2, gamma, beta, eps, want_stats=True):
     """x2 (R, C) rows -> y (R, C), stats (3, R) for frame_norm_bwd (None unless wanted); see ctn_frame_norm_fwd."""
-    lib = _lib.load()
-    code, wcode = _frame_norm_param_type(x2, gamma, beta)
-    if not x2.is_cuda:
-        _require_cuda(x2)
+    code, wcode = _frame_norm_types(x2, gamma, beta)
     R, Cc = x2.shape
     y = x2.new_empty((R, Cc))
     stats = x2.new_empty((3, R), dtype=torch.float32) if want_stats else None
-    _enqueue("ctn_frame_norm_fwd", x2.get_device(), lib.ctn_frame_norm_fwd, x2.data_ptr(), x2.stride(0) if R > 1 else Cc, R, Cc,
-             code, _ptr(gamma), _ptr(beta), wcode, eps, y.data_ptr(), Cc, _ptr(stats))
+    _enqueue("ctn_frame_norm_fwd", x2.get_device(), (_lib._lib or _lib.load()).ctn_frame_norm_fwd, x2.data_ptr(),
+             x2.stride(0) if R > 1 else Cc, R, Cc, code, None if gamma is None else gamma.data_ptr(),
+             None if beta is None else beta.data_ptr(), wcode, eps, y.data_ptr(), Cc, None if stats is None else stats.data_ptr())
     return y, stats
 
 
 def frame_norm_bwd(dy2, x2, gamma, stats, want_dx=True, want_dgamma=None, want_dbeta=None):
     """-> dx (R, C), dgamma (C,), dbeta (C,), each None unless wanted (want_dgamma / want_dbeta: the parameter's dtype);
     see ctn_frame_norm_bwd."""
-    lib = _lib.load()
     R, Cc = x2.shape
-    code = _type(x2, "frame_norm")
-    assert dy2.shape == x2.shape and dy2.dtype == x2.dtype and dy2.device == x2.device
+    code = _TYPES[x2.dtype]
+    assert dy2.shape == x2.shape and dy2.dtype is x2.dtype and dy2.get_device() == x2.get_device()
     wdtype = want_dgamma or want_dbeta or (torch.float32 if gamma is None else gamma.dtype)
     dx = x2.new_empty((R, Cc)) if want_dx else None
+    need = _frame_norm_ws(R, Cc, code) if want_dgamma or want_dbeta else 0
     dgamma = x2.new_empty((Cc,), dtype=wdtype) if want_dgamma else None
     dbeta = x2.new_empty((Cc,), dtype=wdtype) if want_dbeta else None
-    need = _frame_norm_ws(R, Cc, code) if want_dgamma or want_dbeta else 0
     ws = x2.new_empty((need,), dtype=torch.float32) if need else None
-    _enqueue("ctn_frame_norm_bwd", x2.get_device(), lib.ctn_frame_norm_bwd, dy2.data_ptr(), dy2.stride(0) if R > 1 else Cc,
-             x2.data_ptr(), x2.stride(0) if R > 1 else Cc, R, Cc, code, _ptr(gamma), _TYPES[wdtype], stats.data_ptr(), _ptr(dx), Cc,
-             _ptr(dgamma), _ptr(dbeta), _ptr(ws), need)
+    _enqueue("ctn_frame_norm_bwd", x2.get_device(), (_lib._lib or _lib.load()).ctn_frame_norm_bwd, dy2.data_ptr(),
+             dy2.stride(0) if R > 1 else Cc, x2.data_ptr(), x2.stride(0) if R > 1 else Cc, R, Cc, code,
+             None if gamma is None else gamma.data_ptr(), _TYPES[wdtype], stats.data_ptr(), None if dx is None else dx.data_ptr(),
+             Cc, None if dgamma is None else dgamma.data_ptr(), None if dbeta is None else dbeta.data_ptr(),
+             None if ws is None else ws.data_ptr(), need)
     return dx, dgamma, dbeta
 
 

@@ -105,7 +105,7 @@ def test_norm_and_rotary_c_entries_refuse():
     bwd = lambda **o: lib.ctn_frame_norm_bwd(*[{**dict(dy=p, ldd=8, x=p, ldx=8, R=4, C=8, t=0, g=p, w=0, st=p, dx=p, lx=8, dg=p,
                                                        db=p, ws=p, n=0, s=None), **o}[n]
                                                for n in "dy ldd x ldx R C t g w st dx lx dg db ws n s".split()])
-    for over in (dict(), dict(ws=None, n=1 << 20), dict(st=None), dict(t=3), dict(lx=7), dict(C=20000)):
+    for over in (dict(R=400), dict(R=400, ws=None, n=1 << 20), dict(st=None), dict(t=3), dict(lx=7), dict(C=20000)):
         assert bwd(**over) == -1, over
     rot = lambda **o: lib.ctn_rotary(*[{**dict(x=p, xb=64, xt=16, xh=8, B=2, T=4, H=2, D=8, t=0, pos=None, pb=0, first=0, tu=p,
                                                R=8, i=0, inv=0, m=1.0, y=p, yb=64, yt=16, yh=8, s=None), **o}[n]
