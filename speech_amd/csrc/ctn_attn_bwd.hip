@@ -39,7 +39,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
     unsigned tile, unit;
-    deal(blockIdx.x, a.batch * a.H, f.nt, a.causal, tile, unit);
+    deal(blockIdx.x, a.batch * a.H, f.nt, a.causal, a.lengths != nullptr, tile, unit);
     const int qt = f.nt - 1 - (int)tile;                         // with a causal mask the last queries see the most keys
     const int head = unit % a.H, b = unit / a.H, hk = head / f.G;
     const int w0 = qt * 32 * NW + wave * 32, tq = w0 + (lane & 31);
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
     unsigned tile, unit;
-    deal(blockIdx.x, a.batch * a.Hk, f.nt * f.nsplit, a.causal, tile, unit);
+    deal(blockIdx.x, a.batch * a.Hk, f.nt * f.nsplit, a.causal, a.lengths != nullptr, tile, unit);
     const int sp = tile % f.nsplit, kt = tile / f.nsplit;        // with a causal mask the first keys are seen most
     const int hk = unit % a.Hk, b = unit / a.Hk;
     const int b0 = kt * 32 * NW, w0 = b0 + wave * 32, key = w0 + (lane & 31);
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     const bool causal = a.causal != 0;
     const float sl2 = f.sl2, scale = a.scale;
     unsigned tile0, unit;
-    deal(blockIdx.x, gridDim.x, 1, false, tile0, unit);
+    deal(blockIdx.x, gridDim.x, 1, false, a.lengths != nullptr, tile0, unit);
     const int hk = unit % a.Hk, b = unit / a.Hk;
     int len = a.Tk;
     if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);

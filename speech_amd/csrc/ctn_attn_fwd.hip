@@ -36,7 +36,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int off = a.Tk - a.Tq;
     unsigned tile, unit;
-    deal(blockIdx.x, a.batch * f.heads, f.nqt, a.causal, tile, unit);
+    deal(blockIdx.x, a.batch * f.heads, f.nqt, a.causal, a.lengths != nullptr, tile, unit);
     const int qt = f.nqt - 1 - (int)tile;                        // with a causal mask the last queries see the most keys
     const int hh = unit % f.heads, b = unit / f.heads;
 
