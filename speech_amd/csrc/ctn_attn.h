@@ -89,6 +89,11 @@ template <> struct Chunk<float> {
         floats(x);
         make_frag(x, f);
     }
+    // the same, kept inside the loop it stands in (the compiler would otherwise hold the pieces of every pass in registers)
+    __device__ __forceinline__ void frag_again(Frag<3>& f) {
+        asm volatile("" : "+v"(a), "+v"(b));
+        frag(f);
+    }
 };
 
 // LDS image of a plane of rows of DT bf16: the 16-byte chunk ch of row r lies at chunk ch ^ key(r) of its row.  The keys

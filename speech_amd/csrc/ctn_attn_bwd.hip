@@ -10,341 +10,12 @@
 // For bf16 tensors p and ds are rounded to bf16 (half a step, relative 2^-8 each at most) where they enter a product, which
 // adds about as much to a gradient as its own rounding does; in heads of up to 32 features, whose dq also feels what
 // the forward pass's roundings did to delta, dq takes ds in two pieces.
-#include "ctn_attn.h"
+#include "ctn_attn_bwd.h"
 
 bool ctn_attn_args_ok(const ctn_attn_args* a, const char* who);
 
 namespace {
 using namespace attn;
-
-// rows of the walked tiles: 64, or 32 where two buffers of 64 would take more than half of the LDS
-template <typename T, int DT> constexpr int walk_tile() { return Planes<T>::N * DT <= 128 ? 64 : 32; }
-
-struct bwd_params {
-    ctn_attn_args a;
-    int G, nt;               // tiles of the kept axis per (batch element, head)
-    int nsplit;              // dK / dV: pieces of the walk over queries
-    float sl2;
-    float* delta;            // [B][H][Tq]
-    float* part;             // nsplit > 1: [nsplit][dk, dv][B][Tk][Hk][D]
-};
-
-template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_dq_kernel(const bwd_params f) {
-    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, KT = walk_tile<T, DT>();
-    typedef Tile<T, DT, KT, NT> tile_t;
-    constexpr int BUF = 2 * tile_t::BYTES;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
-    const ctn_attn_args& a = f.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int off = a.Tk - a.Tq;
-    unsigned tile, unit;
-    deal(blockIdx.x, a.batch * a.H, f.nt, a.causal, a.lengths != nullptr, tile, unit);
-    const int qt = f.nt - 1 - (int)tile;                         // with a causal mask the last queries see the most keys
-    const int head = unit % a.H, b = unit / a.H, hk = head / f.G;
-    const int w0 = qt * 32 * NW + wave * 32, tq = w0 + (lane & 31);
-    const bool live = tq < a.Tq;
-
-    int len = a.Tk;
-    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
-    const int vis = !live ? 0 : a.causal ? min(len, tq + off + 1) : len;
-    int kend = len, wfull = len, wend = len;
-    if (a.causal) {
-        kend = min(len, min(a.Tq, (qt + 1) * 32 * NW) + off);
-        wfull = min(len, w0 + off + 1);
-        wend = min(len, min(a.Tq, w0 + 32) + off);
-    }
-    if (w0 >= a.Tq) wend = 0;
-    const int t1 = kend > 0 ? (kend + KT - 1) / KT : 0;
-
-    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h;
-    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h;
-    const int64_t kstep = KT * a.k_t, vstep = KT * a.v_t;
-    int left = kend;
-    tile_t tk, tv;
-    tk.init(a.k_t, a.D, threadIdx.x);
-    tv.init(a.v_t, a.D, threadIdx.x);
-    auto fetch = [&]() {                                         // the next tile
-        tk.load(kp, left, a.D);
-        tv.load(vp, left, a.D);
-        kp += kstep, vp += vstep, left -= KT;
-    };
-    auto stage = [&](const int buf) {
-        tk.store(lds + buf * BUF, threadIdx.x);
-        tv.store(lds + buf * BUF + tile_t::BYTES, threadIdx.x);
-    };
-    if (t1 > 0) fetch();
-
-    Frag<NP> q[KS], g[KS];
-    float delta = 0.f;
-    {
-        const T* qp = (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
-        const T* gp = (const T*)a.d_o + b * a.do_b + tq * a.do_t + head * a.do_h;
-        const int64_t at = b * a.o_b + tq * a.o_t + head * a.o_h;
-        Chunk<T> cq[KS], cg[KS], co[KS], cl[NP == 1 ? KS : 1];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = 16 * s + 8 * half;
-            if (live && d < a.D) cq[s].load(qp + d), cg[s].load(gp + d), co[s].load((const T*)a.o + at + d);
-            else cq[s].zero(), cg[s].zero(), co[s].zero();
-        }
-        if constexpr (NP == 1) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int d = 16 * s + 8 * half;
-                if (a.o_low != nullptr && live && d < a.D) cl[s].load((const T*)a.o_low + at + d);
-                else cl[s].zero();
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            cq[s].frag(q[s]);
-            cg[s].frag(g[s]);
-            float x[8], y[8];
-            cg[s].floats(x);
-            co[s].floats(y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
-            if constexpr (NP == 1) {
-                cl[s].floats(y);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
-            }
-        }
-    }
-    delta = half_sum(delta);
-    const int64_t row = ((int64_t)b * a.H + head) * a.Tq + tq;
-    float lse = live ? a.lse[row] : INFINITY;
-    if (lse == -INFINITY) lse = INFINITY;            // a row that sees nothing: every probability comes out as zero
-    if (live && half == 0) f.delta[row] = delta;
-
-    f32x16 dq[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
-    if (t1 > 0) stage(0);
-    __syncthreads();
-    for (int t = 0; t < t1; ++t) {
-        const unsigned char* K = lds + (t & 1) * BUF;
-        const unsigned char* V = K + tile_t::BYTES;
-        if (t + 1 < t1) fetch();
-#pragma unroll
-        for (int r0 = 0; r0 < KT; r0 += 32) {
-            const int k0 = t * KT + r0;
-            if (k0 >= wend) break;
-            f32x16 s, p;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = p[e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                Frag<NP> k, v;
-                frag_rows<NP, DT, KT>(K, r0, i, k);
-                mma(s, k, q[i]);
-                frag_rows<NP, DT, KT>(V, r0, i, v);
-                mma(p, v, g[i]);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f.sl2, -lse)) * (p[e] - delta);
-            if (k0 + 32 > wfull) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = k0 + acc_row(e) < vis ? s[e] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[8 * i + e];
-                Frag<NP> ds, low;
-                make_frag(x, ds);
-                if constexpr (NP == 1 && DT == 32) {             // narrow heads: what the rounding left over as well
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] -= (float)ds.p[0][e];
-                    make_frag(x, low);
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    Frag<NP> k;
-                    frag_cols<NP, DT, KT>(K, r0 + 16 * i, 32 * d, k);
-                    if constexpr (NP == 1 && DT == 32) mma(dq[d], k, low);
-                    mma(dq[d], k, ds);
-                }
-            }
-        }
-        if (t + 1 < t1) stage((t + 1) & 1);
-        __syncthreads();
-    }
-    if (!live || a.dq == nullptr) return;
-    T* dst = (T*)a.dq + b * a.dq_b + tq * a.dq_t + head * a.dq_h;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int c = 32 * d + acc_row(e);
-            if (c < a.D) store4(dst + c, f32x4{dq[d][e], dq[d][e + 1], dq[d][e + 2], dq[d][e + 3]} * a.scale);
-        }
-}
-
-template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2))) void attn_dkv_kernel(const bwd_params f) {
-    constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
-    typedef Tile<T, DT, QT, NT> tile_t;
-    constexpr int BUF = 2 * tile_t::BYTES + 2 * QT * 4;          // Q planes, dO planes, log-sums, deltas
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
-    const ctn_attn_args& a = f.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int off = a.Tk - a.Tq;
-    unsigned tile, unit;
-    deal(blockIdx.x, a.batch * a.Hk, f.nt * f.nsplit, a.causal, a.lengths != nullptr, tile, unit);
-    const int sp = tile % f.nsplit, kt = tile / f.nsplit;        // with a causal mask the first keys are seen most
-    const int hk = unit % a.Hk, b = unit / a.Hk;
-    const int b0 = kt * 32 * NW, w0 = b0 + wave * 32, key = w0 + (lane & 31);
-
-    int len = a.Tk;
-    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
-    const bool seen = key < len;
-    // query q sees key j when j <= q + off: block's and wave's first query, and the wave's first query without a mask
-    const int first = a.causal ? max(0, b0 - off) : 0, wfirst = a.causal ? max(0, w0 - off) : 0;
-    const int wfull = w0 + 32 > len ? a.Tq : a.causal ? w0 + 31 - off : 0;
-    const int t0 = first / QT;
-    const int nq = b0 < len && a.Tq > first ? (a.Tq + QT - 1) / QT - t0 : 0;      // query tiles per head
-    const int i0 = (int)((int64_t)nq * f.G * sp / f.nsplit), i1 = (int)((int64_t)nq * f.G * (sp + 1) / f.nsplit);
-
-    Frag<NP> k[KS], v[KS];
-    {
-        const T* kp = (const T*)a.k + b * a.k_b + key * a.k_t + hk * a.k_h;
-        const T* vp = (const T*)a.v + b * a.v_b + key * a.v_t + hk * a.v_h;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = 16 * s + 8 * half;
-            Chunk<T> ck, cv;
-            if (seen && d < a.D) ck.load(kp + d), cv.load(vp + d);
-            else ck.zero(), cv.zero();
-            ck.frag(k[s]);
-            cv.frag(v[s]);
-        }
-    }
-
-    tile_t tq, tg;
-    tq.init(a.q_t, a.D, threadIdx.x);
-    tg.init(a.do_t, a.D, threadIdx.x);
-    constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
-    float stat[NS];
-    auto fetch = [&](const int i) {
-        const int head = hk * f.G + i / nq, q0 = (t0 + i % nq) * QT;
-        tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.Tq - q0, a.D);
-        tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.Tq - q0, a.D);
-#pragma unroll
-        for (int x = 0; x < NS; ++x) {
-            const int j = threadIdx.x + NT * x, r = q0 + j % QT;
-            const int64_t row = ((int64_t)b * a.H + head) * a.Tq + r;
-            if (j < QT) {
-                stat[x] = r < a.Tq ? a.lse[row] : INFINITY;
-                if (stat[x] == -INFINITY) stat[x] = INFINITY;    // sees nothing: every probability comes out as zero
-            } else if (j < 2 * QT) {
-                stat[x] = r < a.Tq ? f.delta[row] : 0.f;
-            }
-        }
-    };
-    auto stage = [&](const int buf) {
-        unsigned char* p = lds + buf * BUF;
-        tq.store(p, threadIdx.x);
-        tg.store(p + tile_t::BYTES, threadIdx.x);
-#pragma unroll
-        for (int x = 0; x < NS; ++x)
-            if (threadIdx.x + NT * x < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[threadIdx.x + NT * x] = stat[x];
-    };
-    f32x16 dk[ND], dv[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
-    if (i0 < i1) {
-        fetch(i0);
-        stage(0);
-    }
-    __syncthreads();
-    for (int i = i0; i < i1; ++i) {
-        const unsigned char* Q = lds + ((i - i0) & 1) * BUF;
-        const unsigned char* G = Q + tile_t::BYTES;
-        const float* st = reinterpret_cast<const float*>(G + tile_t::BYTES);
-        if (i + 1 < i1) fetch(i + 1);
-#pragma unroll
-        for (int r0 = 0; r0 < QT; r0 += 32) {
-            const int q0 = (t0 + i % nq) * QT + r0;
-            if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
-            f32x16 s, p;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = p[e] = 0.f;
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                Frag<NP> x;
-                frag_rows<NP, DT, QT>(Q, r0, j, x);
-                mma(s, x, k[j]);
-                frag_rows<NP, DT, QT>(G, r0, j, x);
-                mma(p, x, v[j]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x4 lse = ctn_ld4(st + r0 + 8 * r + 4 * half), delta = ctn_ld4(st + QT + r0 + 8 * r + 4 * half);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * r + e], f.sl2, -lse[e]));
-                    s[4 * r + e] = w;
-                    p[4 * r + e] = w * (p[4 * r + e] - delta[e]);
-                }
-            }
-            if (q0 < wfull) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const bool on = seen && (!a.causal || key <= q0 + acc_row(e) + off);
-                    s[e] = on ? s[e] : 0.f;
-                    p[e] = on ? p[e] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float x[8], y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[8 * j + e], y[e] = p[8 * j + e];
-                Frag<NP> w, ds;
-                make_frag(x, w);
-                make_frag(y, ds);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    Frag<NP> c;
-                    frag_cols<NP, DT, QT>(G, r0 + 16 * j, 32 * d, c);
-                    mma(dv[d], c, w);
-                    frag_cols<NP, DT, QT>(Q, r0 + 16 * j, 32 * d, c);
-                    mma(dk[d], c, ds);
-                }
-            }
-        }
-        if (i + 1 < i1) stage((i - i0 + 1) & 1);
-        __syncthreads();
-    }
-    if (key >= a.Tk) return;
-    T* pk = (T*)a.dk + b * a.dk_b + key * a.dk_t + hk * a.dk_h;
-    T* pv = (T*)a.dv + b * a.dv_b + key * a.dv_t + hk * a.dv_h;
-    const int64_t one = (int64_t)a.batch * a.Tk * a.Hk * a.D;
-    float* part = f.part + 2 * sp * one + (((int64_t)b * a.Tk + key) * a.Hk + hk) * a.D;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int c = 32 * d + acc_row(e);
-            if (c >= a.D) continue;
-            const f32x4 x = f32x4{dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]} * a.scale;
-            const f32x4 y = f32x4{dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]};
-            if (f.nsplit > 1) {
-                ctn_st4(part + c, x);
-                ctn_st4(part + one + c, y);
-            } else {
-                if (a.dk) store4(pk + c, x);
-                if (a.dv) store4(pv + c, y);
-            }
-        }
-}
 
 // ------------------------------------------------------------------------------------------------ one block per key head
 // Many short fp32 sequences with heads of up to 32 features (the dual-path blocks: thousands of (sequence, head) pairs of a
@@ -636,22 +307,11 @@ bool whole_fits(const ctn_attn_args& a) {
 int64_t round16(const int64_t n) { return (n + 15) / 16 * 16; }
 int waves_for(const int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 
-template <typename T, int DT>
-void launch_dq(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
-    if (nw == 1) hipLaunchKernelGGL((attn_dq_kernel<T, DT, 1>), dim3(grid), dim3(64), 0, s, f);
-    else if (nw == 2) hipLaunchKernelGGL((attn_dq_kernel<T, DT, 2>), dim3(grid), dim3(128), 0, s, f);
-    else hipLaunchKernelGGL((attn_dq_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
-}
-template <typename T, int DT>
-void launch_dkv(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
-    if (nw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 1>), dim3(grid), dim3(64), 0, s, f);
-    else if (nw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 2>), dim3(grid), dim3(128), 0, s, f);
-    else hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
-}
 template <typename T>
 void launch_bwd(const bool keys, const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
     if (f.a.D <= 32) keys ? launch_dkv<T, 32>(f, nw, grid, s) : launch_dq<T, 32>(f, nw, grid, s);
     else if (f.a.D <= 64) keys ? launch_dkv<T, 64>(f, nw, grid, s) : launch_dq<T, 64>(f, nw, grid, s);
+    else if constexpr (Planes<T>::N == 3) launch_wide(keys, f, nw, grid, s);
     else keys ? launch_dkv<T, 128>(f, nw, grid, s) : launch_dq<T, 128>(f, nw, grid, s);
 }
 
