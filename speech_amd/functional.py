@@ -653,6 +653,32 @@ class AttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
+class RotarySelfAttentionFn(torch.autograd.Function):
+    """Self-attention of a fused projection qkv (N, T, 3 H, D) -- query, key and value heads -- with rotary positions 0 .. T - 1:
+    RotaryFn on the first 2 H heads and AttentionFn, with the gradient of qkv written in place instead of summed from
+    its parts."""
+
+    @staticmethod
+    def forward(ctx, qkv, turns, magnitude, lengths, causal):
+        H = qkv.shape[2] // 3
+        qk, v = ops.rotary(qkv[:, :, :2 * H], turns, magnitude=magnitude), qkv[:, :, 2 * H:]
+        o, lse, low = ops.attn_fwd(qk[:, :, :H], qk[:, :, H:], v, lengths, causal)
+        ctx.save_for_backward(qk, qkv, turns, o, lse, low, lengths)
+        ctx.meta = (magnitude, causal)
+        return o
+
+    @_differentiated_once
+    def backward(ctx, do):
+        qk, qkv, turns, o, lse, low, lengths = ctx.saved_tensors
+        magnitude, causal = ctx.meta
+        H = qkv.shape[2] // 3
+        dqkv, dqk = torch.empty_like(qkv, memory_format=torch.contiguous_format), torch.empty_like(qk)
+        ops.attn_bwd(do, qk[:, :, :H], qk[:, :, H:], qkv[:, :, 2 * H:], o, lse, low, lengths, causal,
+                     out=(dqk[:, :, :H], dqk[:, :, H:], dqkv[:, :, 2 * H:]))
+        ops.rotary(dqk, turns, inverse=True, magnitude=magnitude, out=dqkv[:, :, :2 * H])
+        return dqkv, None, None, None, None
+
+
 # ------------------------------------------------------------------------------------------------ axis shuffles of the dual-path blocks
 class RowsFromBlocksFn(torch.autograd.Function):
     """(B, F, S, K) -> the recurrence's rows (B*S, K, F) (walk_chunks False) or (B*K, S, F) (True), i.e.

@@ -7,7 +7,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from ..functional import AttentionFn, LinearFn, RotaryFn
+from ..functional import AttentionFn, LinearFn, RotaryFn, RotarySelfAttentionFn
 
 
 def attention(q, k, v, lengths=None, causal=False, scale=None):
@@ -122,6 +122,5 @@ class SelfAttention(nn.Module):
         N, T, _ = input.size()
         H, D = self.num_heads, self.head_dim
         qkv = LinearFn.apply(input, self.in_proj.weight, self.in_proj.bias).view(N, T, 3 * H, D)
-        qk = self.rotary(qkv[:, :, :2 * H])
-        out = attention(qk[:, :, :H], qk[:, :, H:], qkv[:, :, 2 * H:], lengths=lengths, causal=self.causal)
+        out = RotarySelfAttentionFn.apply(qkv, self.rotary.turns, self.rotary.magnitude, lengths, self.causal)
         return out.view(N, T, H * D)

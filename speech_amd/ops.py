@@ -459,9 +459,9 @@ def frame_norm_bwd(dy2, x2, gamma, stats, want_dx=True, want_dgamma=None, want_d
     return dx, dgamma, dbeta
 
 
-def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, magnitude=1.0):
-    """x (B, T, H, D) with its leading 2 * turns.numel() elements per head rotated -> dense (B, T, H, D); see ctn_rotary.
-    turns: float64 on x's device; positions: int64 (T,) or (B, T), None: first, first + 1, ..."""
+def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, magnitude=1.0, out=None):
+    """x (B, T, H, D) with its leading 2 * turns.numel() elements per head rotated -> dense (B, T, H, D), or `out` (unit feature
+    stride); see ctn_rotary.  turns: float64 on x's device; positions: int64 (T,) or (B, T), None: first, first + 1, ..."""
     lib = _lib.load()
     _same_place("rotary", x, turns, positions)
     code = _type(x, "rotary")
@@ -486,9 +486,13 @@ def rotary(x, turns, positions=None, first=0, interleaved=False, inverse=False, 
     if xd != 1 and D != 1:
         x = x.contiguous()
         xb, xt, xh, xd = x.stride()
-    y = x.new_empty(shape)
+    if out is None:
+        y, ys = x.new_empty(shape), (T * H * D, H * D, D)
+    else:
+        assert out.shape == shape and out.dtype == x.dtype and out.device == x.device and (D == 1 or out.stride(3) == 1)
+        y, ys = out, out.stride()[:3]
     _enqueue("ctn_rotary", x.get_device(), lib.ctn_rotary, x.data_ptr(), xb, xt, xh, B, T, H, D, code, pptr, pbs, first,
-             turns.data_ptr(), 2 * pairs, 1 if interleaved else 0, 1 if inverse else 0, magnitude, y.data_ptr(), T * H * D, H * D, D)
+             turns.data_ptr(), 2 * pairs, 1 if interleaved else 0, 1 if inverse else 0, magnitude, y.data_ptr(), *ys)
     return y
 
 
@@ -581,8 +585,9 @@ def attn_fwd(q, k, v, lengths=None, causal=False, scale=None, want_lse=True):
     return o, lse, low
 
 
-def attn_bwd(do, q, k, v, o, lse, low, lengths=None, causal=False, scale=None, want=(True, True, True)):
-    """-> dq, dk, dv (dense, each None unless wanted) from the gradient of o and what attn_fwd returned; see ctn_attn_bwd."""
+def attn_bwd(do, q, k, v, o, lse, low, lengths=None, causal=False, scale=None, want=(True, True, True), out=(None, None, None)):
+    """-> dq, dk, dv (each None unless wanted; dense, or the tensors given in `out`: as attn_fwd's operands) from the gradient of o
+    and what attn_fwd returned; see ctn_attn_bwd."""
     lib = _lib.load()
     code = check_attention(q, k, v, lengths)
     B, Tq, H, D = qs = q.shape
@@ -593,17 +598,16 @@ def attn_bwd(do, q, k, v, o, lse, low, lengths=None, causal=False, scale=None, w
     v, vb, vt, vh = _attn_operand(v, ks)
     do, gb, gt, gh = _attn_operand(do, qs)
     lengths = _attn_lengths(lengths, Tk)
-    dq = q.new_empty(qs) if want[0] else None
-    dk = q.new_empty(ks) if want[1] else None
-    dv = q.new_empty(ks) if want[2] else None
+    dq, dk, dv = (None if not w else g if g is not None else q.new_empty(s) for w, g, s in zip(want, out, (qs, ks, ks)))
     need = _attn_ws(B, Tq, Tk, H, Hk, D, code, lengths is not None, True)
     ws = q.new_empty((need,), dtype=torch.float32) if need else None
-    dense_k = (Tk * Hk * D, Hk * D, D)
+    dense_q, dense_k = (Tq * H * D, H * D, D), (Tk * Hk * D, Hk * D, D)
+    gq, gk, gv = (d if g is None else g.stride()[:3] for g, d in zip(out, (dense_q, dense_k, dense_k)))
     args = _lib.AttnArgs.from_buffer_copy(_ATTN_PACK(
         B, Tq, Tk, H, Hk, D, code, 1 if causal else 0, D ** -0.5 if scale is None else scale, 0, _ptr(lengths) or 0,
         q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, o.data_ptr(), Tq * H * D, H * D, D,
-        _ptr(low) or 0, lse.data_ptr(), do.data_ptr(), gb, gt, gh, _ptr(dq) or 0, Tq * H * D, H * D, D, _ptr(dk) or 0, *dense_k,
-        _ptr(dv) or 0, *dense_k, _ptr(ws) or 0, need))
+        _ptr(low) or 0, lse.data_ptr(), do.data_ptr(), gb, gt, gh, _ptr(dq) or 0, *gq, _ptr(dk) or 0, *gk,
+        _ptr(dv) or 0, *gv, _ptr(ws) or 0, need))
     _enqueue("ctn_attn_bwd", q.get_device(), lib.ctn_attn_bwd, args)
     return dq, dk, dv
 

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import attention_cases as ref
+from speech_amd._lib import CtnError
 from speech_amd.modules.attention import RotaryPositions, SelfAttention, attention, rotary_turns, rotate
 from speech_amd.modules.norm import FrameLayerNorm, frame_layer_norm
 
@@ -381,6 +382,56 @@ def test_norm_projection_rotary_attention_together():
     assert rel(xd.grad, x64.grad) < 1e-4
     for n, p in list(norm.named_parameters()) + list(att.named_parameters()):
         assert rel(p.grad, params[n].grad) < 1e-4, n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,causal,D", [(3, True, 16), (600, False, 16), (3, False, 24)])
+def test_fused_projection_equals_its_parts(N, causal, D, dtype):
+    """RotarySelfAttentionFn runs the very kernels that rotate and attention run on the parts: the same bits."""
+    from speech_amd.functional import RotarySelfAttentionFn
+    T, H = 45, 2
+    turns = rotary_turns(D)[0].to(DEV)
+    qkv, do = normal((N, T, 3 * H, D), 1, dtype).to(DEV), normal((N, T, H, D), 2, dtype).to(DEV)
+    lens = torch.randint(0, T + 1, (N,), generator=torch.Generator().manual_seed(1)).to(DEV)
+    a = qkv.clone().requires_grad_(True)
+    ya = RotarySelfAttentionFn.apply(a, turns, 1.5, lens, causal)
+    ya.backward(do)
+    b = qkv.clone().requires_grad_(True)
+    qk = rotate(b[:, :, :2 * H], turns, magnitude=1.5)
+    yb = attention(qk[:, :, :H], qk[:, :, H:], b[:, :, 2 * H:], lens, causal)
+    yb.backward(do)
+    assert torch.equal(ya, yb) and torch.equal(a.grad, b.grad)
+
+
+def test_second_derivatives_are_refused():
+    """autograd.grad calls x unreachable from its gradient, backward() names the reason: an error either way."""
+    x = normal((4, 9, 2, 16), 1).to(DEV).requires_grad_(True)
+    turns = rotary_turns(16)[0].to(DEV)
+    for f in (lambda t: attention(t, t, t), lambda t: rotate(t, turns), lambda t: frame_layer_norm(t)):
+        g, = torch.autograd.grad(f(x).square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="not have been used"):
+            torch.autograd.grad(g.sum(), x)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_other_types_are_refused():
+    turns = rotary_turns(16)[0].to(DEV)
+    for dtype in (torch.float16, torch.float64):
+        x = torch.zeros((1, 2, 2, 16), device=DEV, dtype=dtype)
+        for f in (lambda: attention(x, x, x), lambda: rotate(x, turns), lambda: frame_layer_norm(x)):
+            with pytest.raises(CtnError, match="float32 or bfloat16"):
+                f()
+    x = torch.zeros((1, 2, 2, 16), device=DEV)
+    for f in (lambda: frame_layer_norm(x, torch.ones(16, device=DEV, dtype=BF16)), lambda: frame_layer_norm(x, torch.ones(15, device=DEV)),
+              lambda: frame_layer_norm(x, torch.ones(16)), lambda: rotate(x, turns.cpu()), lambda: rotate(x, turns.float()),
+              lambda: rotate(x, rotary_turns(18)[0].to(DEV)), lambda: rotate(x[0], turns),
+              lambda: rotate(x, turns, torch.zeros(3, device=DEV, dtype=torch.int64)),
+              lambda: rotate(x, turns, torch.zeros(2, device=DEV)), lambda: rotate(x, turns, torch.arange(2)),
+              lambda: attention(x, x, x, lengths=torch.tensor([1])), lambda: attention(x, x, x, scale=0.0),
+              lambda: frame_layer_norm(torch.zeros((1, 16385), device=DEV)), lambda: frame_layer_norm(x, eps=-1.0)):
+        with pytest.raises(CtnError):
+            f()
 
 
 def test_captured_steps_replay_like_eager_ones():

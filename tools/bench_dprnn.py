@@ -1,6 +1,6 @@
 """Training-step time of DPRNN-TasNet at the reference recipe's defaults (N=64, L=2, F=64, H=128, K=250, P=125, B=6,
 4 s at 16 kHz): forward + PIT SI-SDR + backward + clip 5 + Adam, with a per-kernel-family split from torch's profiler.
-usage: [batch]"""
+usage: [batch [lstm|attention]]"""
 import os, sys, time
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT); sys.path.insert(0, os.path.join(ROOT, "tests"))
@@ -13,7 +13,8 @@ from speech_amd.utils import synth
 B = int(sys.argv[1]) if len(sys.argv) > 1 else 4
 dev = torch.device("cuda:0")
 torch.manual_seed(111)
-model = DPRNNTasNet(**cases.PAPER).to(dev)
+kw = {"rnn_type": sys.argv[2]} if len(sys.argv) > 2 else {}
+model = DPRNNTasNet(**dict(cases.PAPER, **kw)).to(dev)
 opt = torch.optim.Adam(model.parameters(), lr=1e-3)
 crit = PIT1d(NegSISDR(), 2)
 mix, src = synth.make_batch(B, 2, 64000, 0)
