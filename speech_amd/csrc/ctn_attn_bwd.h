@@ -336,11 +336,187 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
         }
 }
 
+// PAIR COMMENT
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1))) void attn_dkv_pair_kernel(const bwd_params f) {
+    constexpr int NP = Planes<T>::N, NT = NW * 128, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
+    typedef Tile<T, DT, QT, NT> tile_t;
+    constexpr int BUF = 2 * tile_t::BYTES + 2 * QT * 4;          // Q planes, dO planes, log-sums, deltas
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + NW * QT * 32 * 4];
+    const ctn_attn_args& a = f.a;
+    const int lane = threadIdx.x & 63, both = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const bool keys = both >= NW;                                // this wave's gradient: dK, or dV
+    const int wave = keys ? both - NW : both;
+    float* const probs = reinterpret_cast<float*>(lds + 2 * BUF) + wave * QT * 32 + 4 * lane;      // the pair's P, in the accumulators' order
+    const int off = a.Tk - a.Tq;
+    unsigned tile, unit;
+    deal(blockIdx.x, a.batch * a.Hk, f.nt * f.nsplit, a.causal, a.lengths != nullptr, tile, unit);
+    const int sp = tile % f.nsplit, kt = tile / f.nsplit;        // with a causal mask the first keys are seen most
+    const int hk = unit % a.Hk, b = unit / a.Hk;
+    const int b0 = kt * 32 * NW, w0 = b0 + wave * 32, key = w0 + (lane & 31);
+
+    int len = a.Tk;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
+    const bool seen = key < len;
+    // query q sees key j when j <= q + off: block's and wave's first query, and the wave's first query without a mask
+    const int first = a.causal ? max(0, b0 - off) : 0, wfirst = a.causal ? max(0, w0 - off) : 0;
+    const int wfull = w0 + 32 > len ? a.Tq : a.causal ? w0 + 31 - off : 0;
+    const int t0 = first / QT;
+    const int nq = b0 < len && a.Tq > first ? (a.Tq + QT - 1) / QT - t0 : 0;      // query tiles per head
+    const int i0 = (int)((int64_t)nq * f.G * sp / f.nsplit), i1 = (int)((int64_t)nq * f.G * (sp + 1) / f.nsplit);
+
+    Frag<NP> kept[KS];
+    {
+        const T* p = keys ? (const T*)a.v + b * a.v_b + key * a.v_t + hk * a.v_h : (const T*)a.k + b * a.k_b + key * a.k_t + hk * a.k_h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * half;
+            Chunk<T> c;
+            if (seen && d < a.D) c.load(p + d);
+            else c.zero();
+            c.frag(kept[s]);
+        }
+    }
+
+    tile_t tq, tg;
+    tq.init(a.q_t, a.D, threadIdx.x);
+    tg.init(a.do_t, a.D, threadIdx.x);
+    constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
+    float stat[NS];
+    auto fetch = [&](const int i) {
+        const int head = hk * f.G + i / nq, q0 = (t0 + i % nq) * QT;
+        tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.Tq - q0, a.D);
+        tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.Tq - q0, a.D);
+#pragma unroll
+        for (int x = 0; x < NS; ++x) {
+            const int j = threadIdx.x + NT * x, r = q0 + j % QT;
+            const int64_t row = ((int64_t)b * a.H + head) * a.Tq + r;
+            if (j < QT) {
+                stat[x] = r < a.Tq ? a.lse[row] : INFINITY;
+                if (stat[x] == -INFINITY) stat[x] = INFINITY;    // sees nothing: every probability comes out as zero
+            } else if (j < 2 * QT) {
+                stat[x] = r < a.Tq ? f.delta[row] : 0.f;
+            }
+        }
+    };
+    auto stage = [&](const int buf) {
+        unsigned char* p = lds + buf * BUF;
+        tq.store(p, threadIdx.x);
+        tg.store(p + tile_t::BYTES, threadIdx.x);
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+            if (threadIdx.x + NT * x < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[threadIdx.x + NT * x] = stat[x];
+    };
+    f32x16 acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    if (i0 < i1) {
+        fetch(i0);
+        stage(0);
+    }
+    __syncthreads();
+    for (int i = i0; i < i1; ++i) {
+        const unsigned char* const buf = lds + ((i - i0) & 1) * BUF;
+        const unsigned char* const mine = buf + (keys ? tile_t::BYTES : 0);        // multiplies what the wave keeps: dO with V, Q with K
+        const unsigned char* const other = buf + (keys ? 0 : tile_t::BYTES);
+        const float* st = reinterpret_cast<const float*>(buf + 2 * tile_t::BYTES);
+        if (i + 1 < i1) fetch(i + 1);
+        f32x16 s[QT / 32];
+        if (!keys) __builtin_amdgcn_s_setprio(1);                // the exponentials then run beside the other wave's products
+#pragma unroll
+        for (int r = 0; r < QT / 32; ++r) {
+            const int q0 = (t0 + i % nq) * QT + 32 * r;
+            if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[r][e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                Frag<NP> x;
+                frag_rows<NP, DT, QT>(mine, 32 * r, j, x);
+                mma(s[r], x, kept[j]);
+            }
+            if (keys) continue;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 lse = ctn_ld4(st + 32 * r + 8 * g + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[r][4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][4 * g + e], f.sl2, -lse[e]));
+            }
+            if (q0 < wfull) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[r][e] = seen && (!a.causal || key <= q0 + acc_row(e) + off) ? s[r][e] : 0.f;
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                ctn_st4(probs + 1024 * r + 256 * g, f32x4{s[r][4 * g], s[r][4 * g + 1], s[r][4 * g + 2], s[r][4 * g + 3]});
+        }
+        __builtin_amdgcn_s_setprio(0);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < QT / 32; ++r) {
+            const int q0 = (t0 + i % nq) * QT + 32 * r;
+            if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
+            if (keys) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 delta = ctn_ld4(st + QT + 32 * r + 8 * g + 4 * half), w = ctn_ld4(probs + 1024 * r + 256 * g);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[r][4 * g + e] = w[e] * (s[r][4 * g + e] - delta[e]);
+                }
+                if (q0 < wfull) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[r][e] = seen && (!a.causal || key <= q0 + acc_row(e) + off) ? s[r][e] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[r][8 * j + e];
+                Frag<NP> w;
+                make_frag(x, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<NP> c;
+                    frag_cols<NP, DT, QT>(other, 32 * r + 16 * j, 32 * d, c);
+                    mma(acc[d], c, w);
+                }
+            }
+        }
+        if (i + 1 < i1) stage((i - i0 + 1) & 1);
+        __syncthreads();
+    }
+    if (key >= a.Tk) return;
+    const float scale = keys ? a.scale : 1.f;
+    T* const out = keys ? (T*)a.dk + b * a.dk_b + key * a.dk_t + hk * a.dk_h : (T*)a.dv + b * a.dv_b + key * a.dv_t + hk * a.dv_h;
+    const bool wanted = (keys ? a.dk : a.dv) != nullptr;
+    const int64_t one = (int64_t)a.batch * a.Tk * a.Hk * a.D;
+    float* const part = f.part + (2 * sp + (keys ? 0 : 1)) * one + (((int64_t)b * a.Tk + key) * a.Hk + hk) * a.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = 32 * d + acc_row(e);
+            if (c >= a.D) continue;
+            const f32x4 x = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]} * scale;
+            if (f.nsplit > 1) ctn_st4(part + c, x);
+            else if (wanted) store4(out + c, x);
+        }
+}
+
 template <typename T, int DT>
 void launch_dq(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
     if (nw == 1) hipLaunchKernelGGL((attn_dq_kernel<T, DT, 1>), dim3(grid), dim3(64), 0, s, f);
     else if (nw == 2) hipLaunchKernelGGL((attn_dq_kernel<T, DT, 2>), dim3(grid), dim3(128), 0, s, f);
     else hipLaunchKernelGGL((attn_dq_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
+}
+template <typename T, int DT>
+void launch_pair(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
+    if (nw == 1) hipLaunchKernelGGL((attn_dkv_pair_kernel<T, DT, 1>), dim3(grid), dim3(128), 0, s, f);
+    else if (nw == 2) hipLaunchKernelGGL((attn_dkv_pair_kernel<T, DT, 2>), dim3(grid), dim3(256), 0, s, f);
+    else hipLaunchKernelGGL((attn_dkv_pair_kernel<T, DT, 4>), dim3(grid), dim3(512), 0, s, f);
 }
 template <typename T, int DT>
 void launch_dkv(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {

@@ -312,7 +312,7 @@ void launch_bwd(const bool keys, const bwd_params& f, const int nw, const unsign
     if (f.a.D <= 32) keys ? launch_dkv<T, 32>(f, nw, grid, s) : launch_dq<T, 32>(f, nw, grid, s);
     else if (f.a.D <= 64) keys ? launch_dkv<T, 64>(f, nw, grid, s) : launch_dq<T, 64>(f, nw, grid, s);
     else if constexpr (Planes<T>::N == 3) launch_wide(keys, f, nw, grid, s);
-    else keys ? launch_dkv<T, 128>(f, nw, grid, s) : launch_dq<T, 128>(f, nw, grid, s);
+    else keys ? launch_pair<T, 128>(f, nw, grid, s) : launch_dq<T, 128>(f, nw, grid, s);
 }
 
 }  // namespace

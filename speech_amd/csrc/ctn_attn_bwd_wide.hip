@@ -8,7 +8,7 @@
 namespace attn {
 
 void launch_wide(const bool keys, const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
-    if (keys) launch_dkv<float, 128>(f, nw, grid, s);
+    if (keys) launch_pair<float, 128>(f, nw, grid, s);
     else launch_dq<float, 128>(f, nw, grid, s);
 }
 
