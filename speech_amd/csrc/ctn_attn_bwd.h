@@ -218,31 +218,36 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
     tile_t tq, tg;
     tq.init(a.q_t, a.D, threadIdx.x);
     tg.init(a.do_t, a.D, threadIdx.x);
-    constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
+    // The next tile's log-sums, then its deltas: loaded with the tile, looked at when it is stored (looking at a value waits for
+    // every load before it).  fh, ft: the next tile to fetch, ct: the one at hand, counted on from the piece's first.
+    constexpr int NS = (2 * QT + NT - 1) / NT;
     float stat[NS];
-    auto fetch = [&](const int i) {
-        const int head = hk * f.G + i / nq, q0 = (t0 + i % nq) * QT;
+    int fh = nq > 0 ? i0 / nq : 0, ft = nq > 0 ? i0 % nq : 0, ct = ft, fetched = 0;
+    auto fetch = [&]() {
+        const int head = hk * f.G + fh, q0 = (t0 + ft) * QT;
         tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.Tq - q0, a.D);
         tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.Tq - q0, a.D);
+        const int64_t row = ((int64_t)b * a.H + head) * a.Tq;
 #pragma unroll
         for (int x = 0; x < NS; ++x) {
-            const int j = threadIdx.x + NT * x, r = q0 + j % QT;
-            const int64_t row = ((int64_t)b * a.H + head) * a.Tq + r;
-            if (j < QT) {
-                stat[x] = r < a.Tq ? a.lse[row] : INFINITY;
-                if (stat[x] == -INFINITY) stat[x] = INFINITY;    // sees nothing: every probability comes out as zero
-            } else if (j < 2 * QT) {
-                stat[x] = r < a.Tq ? f.delta[row] : 0.f;
-            }
+            const int j = threadIdx.x + NT * x;
+            stat[x] = (j < QT ? a.lse : f.delta)[row + min(q0 + j % QT, a.Tq - 1)];
         }
+        fetched = q0;
+        if (++ft == nq) ft = 0, ++fh;
     };
     auto stage = [&](const int buf) {
         unsigned char* p = lds + buf * BUF;
         tq.store(p, threadIdx.x);
         tg.store(p + tile_t::BYTES, threadIdx.x);
 #pragma unroll
-        for (int x = 0; x < NS; ++x)
-            if (threadIdx.x + NT * x < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[threadIdx.x + NT * x] = stat[x];
+        for (int x = 0; x < NS; ++x) {
+            const int j = threadIdx.x + NT * x;
+            const bool there = fetched + j % QT < a.Tq;
+            // a row that is not there, or sees nothing: every probability comes out as zero
+            const float v = j < QT ? (there && stat[x] != -INFINITY ? stat[x] : INFINITY) : (there ? stat[x] : 0.f);
+            if (j < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[j] = v;
+        }
     };
     f32x16 dk[ND], dv[ND];
 #pragma unroll
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
     if (i0 < i1) {
-        fetch(i0);
+        fetch();
         stage(0);
     }
     __syncthreads();
@@ -258,10 +263,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
         const unsigned char* Q = lds + ((i - i0) & 1) * BUF;
         const unsigned char* G = Q + tile_t::BYTES;
         const float* st = reinterpret_cast<const float*>(G + tile_t::BYTES);
-        if (i + 1 < i1) fetch(i + 1);
+        if (i + 1 < i1) fetch();
 #pragma unroll
         for (int r0 = 0; r0 < QT; r0 += 32) {
-            const int q0 = (t0 + i % nq) * QT + r0;
+            const int q0 = (t0 + ct) * QT + r0;
             if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
             f32x16 s, p;
 #pragma unroll
@@ -311,6 +316,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
             }
         }
         if (i + 1 < i1) stage((i - i0 + 1) & 1);
+        if (++ct == nq) ct = 0;
         __syncthreads();
     }
     if (key >= a.Tk) return;
@@ -336,7 +342,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 1
         }
 }
 
-// PAIR COMMENT
+// The same for heads of 65 to 128 features, where both gradients' accumulators (128 registers for 32 keys), the keys and the
+// values would leave room for one wave a SIMD: the 32 keys belong to a pair of waves, one for dV and one for dK.  The first
+// forms S^T and the probabilities, which it hands to the second through LDS in fp32, the second dP^T and from both the score
+// gradients; either runs half of the products, 32 queries by 128 features at a time, and none is formed twice.  Two barriers a
+// tile: behind the scores, and behind the products that read the tile.  Two waves a SIMD, 32 matrix instructions a wave and
+// tile of 64 queries (bf16): 423 us for one wave with both gradients, 345 us for pairs (bf16, two sequences of 4096 causal
+// steps, 16 heads on 4 of 128 features; 833 TFLOP/s); fp32, 16 sequences of 1024 causal steps, 8 heads on 2: 470 us, 360 us.
+// Giving either wave of a pair the higher priority changes nothing.
 template <typename T, int DT, int NW>
 __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1))) void attn_dkv_pair_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 128, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
@@ -381,31 +394,36 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
     tile_t tq, tg;
     tq.init(a.q_t, a.D, threadIdx.x);
     tg.init(a.do_t, a.D, threadIdx.x);
-    constexpr int NS = (2 * QT + NT - 1) / NT;                   // the next tile's log-sums, then its deltas
+    // The next tile's log-sums, then its deltas: loaded with the tile, looked at when it is stored (looking at a value waits for
+    // every load before it).  fh, ft: the next tile to fetch, ct: the one at hand, counted on from the piece's first.
+    constexpr int NS = (2 * QT + NT - 1) / NT;
     float stat[NS];
-    auto fetch = [&](const int i) {
-        const int head = hk * f.G + i / nq, q0 = (t0 + i % nq) * QT;
+    int fh = nq > 0 ? i0 / nq : 0, ft = nq > 0 ? i0 % nq : 0, ct = ft, fetched = 0;
+    auto fetch = [&]() {
+        const int head = hk * f.G + fh, q0 = (t0 + ft) * QT;
         tq.load((const T*)a.q + b * a.q_b + head * a.q_h + q0 * a.q_t, a.Tq - q0, a.D);
         tg.load((const T*)a.d_o + b * a.do_b + head * a.do_h + q0 * a.do_t, a.Tq - q0, a.D);
+        const int64_t row = ((int64_t)b * a.H + head) * a.Tq;
 #pragma unroll
         for (int x = 0; x < NS; ++x) {
-            const int j = threadIdx.x + NT * x, r = q0 + j % QT;
-            const int64_t row = ((int64_t)b * a.H + head) * a.Tq + r;
-            if (j < QT) {
-                stat[x] = r < a.Tq ? a.lse[row] : INFINITY;
-                if (stat[x] == -INFINITY) stat[x] = INFINITY;    // sees nothing: every probability comes out as zero
-            } else if (j < 2 * QT) {
-                stat[x] = r < a.Tq ? f.delta[row] : 0.f;
-            }
+            const int j = threadIdx.x + NT * x;
+            stat[x] = (j < QT ? a.lse : f.delta)[row + min(q0 + j % QT, a.Tq - 1)];
         }
+        fetched = q0;
+        if (++ft == nq) ft = 0, ++fh;
     };
     auto stage = [&](const int buf) {
         unsigned char* p = lds + buf * BUF;
         tq.store(p, threadIdx.x);
         tg.store(p + tile_t::BYTES, threadIdx.x);
 #pragma unroll
-        for (int x = 0; x < NS; ++x)
-            if (threadIdx.x + NT * x < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[threadIdx.x + NT * x] = stat[x];
+        for (int x = 0; x < NS; ++x) {
+            const int j = threadIdx.x + NT * x;
+            const bool there = fetched + j % QT < a.Tq;
+            // a row that is not there, or sees nothing: every probability comes out as zero
+            const float v = j < QT ? (there && stat[x] != -INFINITY ? stat[x] : INFINITY) : (there ? stat[x] : 0.f);
+            if (j < 2 * QT) reinterpret_cast<float*>(p + 2 * tile_t::BYTES)[j] = v;
+        }
     };
     f32x16 acc[ND];
 #pragma unroll
@@ -413,7 +431,7 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
     if (i0 < i1) {
-        fetch(i0);
+        fetch();
         stage(0);
     }
     __syncthreads();
@@ -422,12 +440,11 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
         const unsigned char* const mine = buf + (keys ? tile_t::BYTES : 0);        // multiplies what the wave keeps: dO with V, Q with K
         const unsigned char* const other = buf + (keys ? 0 : tile_t::BYTES);
         const float* st = reinterpret_cast<const float*>(buf + 2 * tile_t::BYTES);
-        if (i + 1 < i1) fetch(i + 1);
+        if (i + 1 < i1) fetch();
         f32x16 s[QT / 32];
-        if (!keys) __builtin_amdgcn_s_setprio(1);                // the exponentials then run beside the other wave's products
 #pragma unroll
         for (int r = 0; r < QT / 32; ++r) {
-            const int q0 = (t0 + i % nq) * QT + 32 * r;
+            const int q0 = (t0 + ct) * QT + 32 * r;
             if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[r][e] = 0.f;
@@ -452,11 +469,10 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
             for (int g = 0; g < 4; ++g)
                 ctn_st4(probs + 1024 * r + 256 * g, f32x4{s[r][4 * g], s[r][4 * g + 1], s[r][4 * g + 2], s[r][4 * g + 3]});
         }
-        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < QT / 32; ++r) {
-            const int q0 = (t0 + i % nq) * QT + 32 * r;
+            const int q0 = (t0 + ct) * QT + 32 * r;
             if (q0 + 32 <= wfirst || q0 >= a.Tq || w0 >= len) continue;
             if (keys) {
 #pragma unroll
@@ -486,6 +502,7 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
             }
         }
         if (i + 1 < i1) stage((i - i0 + 1) & 1);
+        if (++ct == nq) ct = 0;
         __syncthreads();
     }
     if (key >= a.Tk) return;
