@@ -19,8 +19,6 @@ FLAGS = ["-O3", "--offload-arch=" + ARCH, "-fPIC", "-std=c++17", "-munsafe-fp-at
          "-Wno-unused-function", "-fno-gpu-rdc",
          # no packed fp32 arithmetic: some forms of the instructions give wrong results now and then on this hardware
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# flags of single sources (the reason stands at the top of each)
-SOURCE_FLAGS = {"ctn_attn_bwd_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def sources():
@@ -46,7 +44,7 @@ def build(force=False, verbose=False):
         src, obj = pair
         if not force and not _stale(obj, [src] + headers):
             return None
-        cmd = [hipcc] + FLAGS + SOURCE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
+        cmd = [hipcc] + FLAGS + ["-c", src, "-o", obj]
         if verbose:
             cmd.insert(1, "-Rpass-analysis=kernel-resource-usage")
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,5 +1,4 @@
-// The two launches of attention's backward pass (ctn_attn_bwd.hip has the mathematics); ctn_attn_bwd_wide.hip builds them for
-// fp32 heads of more than 64 features.
+// The two launches of attention's backward pass (ctn_attn_bwd.hip has the mathematics).
 #pragma once
 #include "ctn_attn.h"
 
@@ -18,7 +17,7 @@ struct bwd_params {
 };
 
 template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(Planes<T>::N * DT > 192 ? 1 : 2))) void attn_dq_kernel(const bwd_params f) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_dq_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, KT = walk_tile<T, DT>();
     typedef Tile<T, DT, KT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES;
@@ -175,8 +174,170 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(Planes<
         }
 }
 
+// The same for fp32 heads of 65 to 128 features, whose queries, output gradients (three planes of each) and sums would leave room
+// for one wave a SIMD: 32 queries belong to a pair of waves, one forms the probabilities, the other dP^T - delta.  They
+// exchange the two through LDS in fp32, and each adds the products of one half of the features to its dQ.  16 sequences of 1024
+// causal steps, 8 heads on 2 of 128 features: 312 us, one wave for both 417 us.  (bf16 keys and values are a third as large, and
+// one wave has room for both at two waves a SIMD.)
 template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2))) void attn_dkv_kernel(const bwd_params f) {
+__global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1))) void attn_dq_pair_kernel(const bwd_params f) {
+    constexpr int NP = Planes<T>::N, NT = NW * 128, KS = DT / 16, ND = DT / 64, KT = walk_tile<T, DT>();
+    typedef Tile<T, DT, KT, NT> tile_t;
+    constexpr int BUF = 2 * tile_t::BYTES;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF + 2 * NW * KT * 32 * 4];
+    const ctn_attn_args& a = f.a;
+    const int lane = threadIdx.x & 63, both = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const bool grad = both >= NW;                                // this wave's scores: dO V^T, or Q K^T
+    const int wave = grad ? both - NW : both;
+    float* const factors = reinterpret_cast<float*>(lds + 2 * BUF) + 4 * lane;      // the scores' factors, in the accumulators' order
+    float* const mine = factors + both * KT * 32;
+    const float* const theirs = factors + (grad ? wave : wave + NW) * KT * 32;
+    const int off = a.Tk - a.Tq;
+    unsigned tile, unit;
+    deal(blockIdx.x, a.batch * a.H, f.nt, a.causal, a.lengths != nullptr, tile, unit);
+    const int qt = f.nt - 1 - (int)tile;                         // with a causal mask the last queries see the most keys
+    const int head = unit % a.H, b = unit / a.H, hk = head / f.G;
+    const int w0 = qt * 32 * NW + wave * 32, tq = w0 + (lane & 31);
+    const bool live = tq < a.Tq;
+
+    int len = a.Tk;
+    if (a.lengths) len = min(max(a.lengths[b], 0), a.Tk);
+    const int vis = !live ? 0 : a.causal ? min(len, tq + off + 1) : len;
+    int kend = len, wfull = len, wend = len;
+    if (a.causal) {
+        kend = min(len, min(a.Tq, (qt + 1) * 32 * NW) + off);
+        wfull = min(len, w0 + off + 1);
+        wend = min(len, min(a.Tq, w0 + 32) + off);
+    }
+    if (w0 >= a.Tq) wend = 0;
+    const int t1 = kend > 0 ? (kend + KT - 1) / KT : 0;
+
+    const T* kp = (const T*)a.k + b * a.k_b + hk * a.k_h;
+    const T* vp = (const T*)a.v + b * a.v_b + hk * a.v_h;
+    const int64_t kstep = KT * a.k_t, vstep = KT * a.v_t;
+    int left = kend;
+    tile_t tk, tv;
+    tk.init(a.k_t, a.D, threadIdx.x);
+    tv.init(a.v_t, a.D, threadIdx.x);
+    auto fetch = [&]() {                                         // the next tile
+        tk.load(kp, left, a.D);
+        tv.load(vp, left, a.D);
+        kp += kstep, vp += vstep, left -= KT;
+    };
+    auto stage = [&](const int buf) {
+        tk.store(lds + buf * BUF, threadIdx.x);
+        tv.store(lds + buf * BUF + tile_t::BYTES, threadIdx.x);
+    };
+    if (t1 > 0) fetch();
+
+    Frag<NP> kept[KS];
+    float delta = 0.f;
+    {
+        const T* p = grad ? (const T*)a.d_o + b * a.do_b + tq * a.do_t + head * a.do_h : (const T*)a.q + b * a.q_b + tq * a.q_t + head * a.q_h;
+        const T* op = (const T*)a.o + b * a.o_b + tq * a.o_t + head * a.o_h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * half;
+            Chunk<T> c, o;
+            if (live && d < a.D) c.load(p + d);
+            else c.zero();
+            if (grad && live && d < a.D) o.load(op + d);
+            else o.zero();
+            c.frag(kept[s]);
+            float x[8], y[8];
+            c.floats(x);
+            o.floats(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
+        }
+    }
+    delta = half_sum(delta);
+    const int64_t row = ((int64_t)b * a.H + head) * a.Tq + tq;
+    float lse = live ? a.lse[row] : INFINITY;
+    if (lse == -INFINITY) lse = INFINITY;            // a row that sees nothing: every probability comes out as zero
+    if (grad && live && half == 0) f.delta[row] = delta;
+
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+    if (t1 > 0) stage(0);
+    __syncthreads();
+    for (int t = 0; t < t1; ++t) {
+        const unsigned char* const K = lds + (t & 1) * BUF;
+        const unsigned char* const rows = K + (grad ? tile_t::BYTES : 0);
+        if (t + 1 < t1) fetch();
+        f32x16 s[KT / 32];
+#pragma unroll
+        for (int r = 0; r < KT / 32; ++r) {
+            const int k0 = t * KT + 32 * r;
+            if (k0 >= wend) break;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[r][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                Frag<NP> x;
+                frag_rows<NP, DT, KT>(rows, 32 * r, i, x);
+                mma(s[r], x, kept[i]);
+            }
+            if (grad) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[r][e] -= delta;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[r][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][e], f.sl2, -lse));
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                ctn_st4(mine + 1024 * r + 256 * g, f32x4{s[r][4 * g], s[r][4 * g + 1], s[r][4 * g + 2], s[r][4 * g + 3]});
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < KT / 32; ++r) {
+            const int k0 = t * KT + 32 * r;
+            if (k0 >= wend) break;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = ctn_ld4(theirs + 1024 * r + 256 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[r][4 * g + e] *= x[e];
+            }
+            if (k0 + 32 > wfull) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[r][e] = k0 + acc_row(e) < vis ? s[r][e] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[r][8 * i + e];
+                Frag<NP> ds;
+                make_frag(x, ds);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<NP> k;
+                    frag_cols<NP, DT, KT>(K, 32 * r + 16 * i, 32 * d + (grad ? DT / 2 : 0), k);
+                    mma(dq[d], k, ds);
+                }
+            }
+        }
+        if (t + 1 < t1) stage((t + 1) & 1);
+        __syncthreads();
+    }
+    if (!live || a.dq == nullptr) return;
+    T* dst = (T*)a.dq + b * a.dq_b + tq * a.dq_t + head * a.dq_h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = 32 * d + (grad ? DT / 2 : 0) + acc_row(e);
+            if (c < a.D) store4(dst + c, f32x4{dq[d][e], dq[d][e + 1], dq[d][e + 2], dq[d][e + 3]} * a.scale);
+        }
+}
+
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_dkv_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 64, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
     typedef Tile<T, DT, QT, NT> tile_t;
     constexpr int BUF = 2 * tile_t::BYTES + 2 * QT * 4;          // Q planes, dO planes, log-sums, deltas
@@ -530,7 +691,13 @@ void launch_dq(const bwd_params& f, const int nw, const unsigned grid, hipStream
     else hipLaunchKernelGGL((attn_dq_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
 }
 template <typename T, int DT>
-void launch_pair(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
+void launch_dq_pair(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
+    if (nw == 1) hipLaunchKernelGGL((attn_dq_pair_kernel<T, DT, 1>), dim3(grid), dim3(128), 0, s, f);
+    else if (nw == 2) hipLaunchKernelGGL((attn_dq_pair_kernel<T, DT, 2>), dim3(grid), dim3(256), 0, s, f);
+    else hipLaunchKernelGGL((attn_dq_pair_kernel<T, DT, 4>), dim3(grid), dim3(512), 0, s, f);
+}
+template <typename T, int DT>
+void launch_dkv_pair(const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
     if (nw == 1) hipLaunchKernelGGL((attn_dkv_pair_kernel<T, DT, 1>), dim3(grid), dim3(128), 0, s, f);
     else if (nw == 2) hipLaunchKernelGGL((attn_dkv_pair_kernel<T, DT, 2>), dim3(grid), dim3(256), 0, s, f);
     else hipLaunchKernelGGL((attn_dkv_pair_kernel<T, DT, 4>), dim3(grid), dim3(512), 0, s, f);
@@ -541,8 +708,5 @@ void launch_dkv(const bwd_params& f, const int nw, const unsigned grid, hipStrea
     else if (nw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 2>), dim3(grid), dim3(128), 0, s, f);
     else hipLaunchKernelGGL((attn_dkv_kernel<T, DT, 4>), dim3(grid), dim3(256), 0, s, f);
 }
-
-// ctn_attn_bwd_wide.hip
-void launch_wide(bool keys, const bwd_params& f, int nw, unsigned grid, hipStream_t s);
 
 }  // namespace attn

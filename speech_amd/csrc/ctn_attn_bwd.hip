@@ -290,7 +290,7 @@ __global__ __launch_bounds__(256) void attn_add_kernel(const bwd_params f) {
 // Pieces of the dK / dV walk.  A launch of few blocks ends with its longest one -- a causal mask or few key heads under
 // many query heads make them unequal -- so the walk over (query head, query tile) is cut until there are two blocks a CU,
 // into pieces of four tiles at least.  4096 causal tokens, 16 heads on 4 of 128 features, bf16, two sequences (256 uncut
-// blocks): 1981 us uncut, 654 in two pieces, 677 in four (more sums to store and add).
+// blocks): 560 us uncut, 346 in two pieces, 368 in four (more sums to store and add).
 int dkv_pieces(const ctn_attn_args& a, const int nt) {
     const int64_t blocks = (int64_t)a.batch * a.Hk * nt, tiles = (int64_t)(a.H / a.Hk) * ctn_cdiv(a.Tq, 64);
     if (blocks >= 512) return 1;
@@ -311,8 +311,9 @@ template <typename T>
 void launch_bwd(const bool keys, const bwd_params& f, const int nw, const unsigned grid, hipStream_t s) {
     if (f.a.D <= 32) keys ? launch_dkv<T, 32>(f, nw, grid, s) : launch_dq<T, 32>(f, nw, grid, s);
     else if (f.a.D <= 64) keys ? launch_dkv<T, 64>(f, nw, grid, s) : launch_dq<T, 64>(f, nw, grid, s);
-    else if constexpr (Planes<T>::N == 3) launch_wide(keys, f, nw, grid, s);
-    else keys ? launch_pair<T, 128>(f, nw, grid, s) : launch_dq<T, 128>(f, nw, grid, s);
+    else if (keys) launch_dkv_pair<T, 128>(f, nw, grid, s);
+    else if constexpr (Planes<T>::N == 3) launch_dq_pair<T, 128>(f, nw, grid, s);
+    else launch_dq<T, 128>(f, nw, grid, s);
 }
 
 }  // namespace
