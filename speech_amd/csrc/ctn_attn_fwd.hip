@@ -25,6 +25,7 @@ struct fwd_params {
 // from exact ones as their own rounding without it, 1.42 with it).  A variant of its own because the branch alone costs a
 // long sequence's loop a tenth.
 constexpr int FEW_KEYS = 128, SHORT_KEYS = 512;
+constexpr float SLACK = 8.f;             // doublings over the maximum that a row's sums stand for
 
 template <typename T, int DT, int NW, int KT, bool SHORT>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_fwd_kernel(const fwd_params f) {
@@ -99,7 +100,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    // The sums stand for exponentials over `base`, the row's largest score when they were last scaled.  A larger one rescales the
+    // wave's rows only once its exponential passes 2^SLACK: nothing loses digits below that, and some row of 32 sees a new
+    // maximum in most tiles (8 sequences of 444 to 1777 keys, 12 heads of 64 features, bf16: 85 us rescaled at every maximum, 78 us so).
+    float m = -INFINITY, l = 0.f, base = 0.f, lim = -INFINITY;
+    const float slack = SLACK / f.sl2;
 
     if (ntile > 0) stage(0);
     __syncthreads();
@@ -138,17 +143,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
             for (int j = 0; j < NK; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[j][e]);
-            const float mn = fmaxf(m, half_max(mx));
-            const float base = mn == -INFINITY ? 0.f : mn * f.sl2;           // rows that see nothing yet stay at zero
-            if (__any(mn != m)) {
-                const float alpha = __builtin_amdgcn_exp2f(m * f.sl2 - base);
+            if (__any(mx > lim)) {
+                m = fmaxf(m, half_max(mx));
+                const float next = m == -INFINITY ? 0.f : m * f.sl2;         // rows that see nothing yet stay at zero
+                const float alpha = lim == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - next);
+                base = next, lim = m + slack;
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
             }
-            m = mn;
 #pragma unroll
             for (int i = 0; i < 2 * NK; ++i) {
                 float x[8];
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     l = half_sum(l);
     if (!live) return;
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    const float lse = l > 0.f ? m * f.sl2 + __builtin_amdgcn_logf(l) : -INFINITY;
+    const float lse = l > 0.f ? base + __builtin_amdgcn_logf(l) : -INFINITY;
     const int64_t at = b * a.o_b + tq * a.o_t + head * a.o_h;
 #pragma unroll
     for (int d = 0; d < ND; ++d)

@@ -662,7 +662,7 @@ class RotarySelfAttentionFn(torch.autograd.Function):
     def forward(ctx, qkv, turns, magnitude, lengths, causal):
         H = qkv.shape[2] // 3
         qk, v = ops.rotary(qkv[:, :, :2 * H], turns, magnitude=magnitude), qkv[:, :, 2 * H:]
-        o, lse, low = ops.attn_fwd(qk[:, :, :H], qk[:, :, H:], v, lengths, causal)
+        o, lse, low = ops.attn_fwd(qk[:, :, :H], qk[:, :, H:], v, lengths, causal, want_lse=ctx.needs_input_grad[0])
         ctx.save_for_backward(qk, qkv, turns, o, lse, low, lengths)
         ctx.meta = (magnitude, causal)
         return o

@@ -15,7 +15,8 @@ def attention(q, k, v, lengths=None, causal=False, scale=None):
 
     Key j is visible to query i when j < lengths[b] and, if causal, j <= i + Tk - Tq: the last query sees the last key, so a
     few new queries against all keys so far need no other mask.  A row that sees no key is zero.  Keys and values behind a
-    sequence's length are never read.
+    sequence's length are never read; the causal mask hides scores only, so a NaN or infinity in a later key or value below the
+    length may still reach a query.
 
     Args:
         q (B, Tq, H, D), k and v (B, Tk, Hk, D): float32 or bfloat16, H a multiple of Hk (query heads of a key head are

@@ -248,6 +248,52 @@ def test_attention_of_many_sequences(B, Tq, Tk, H, Hk, D, causal, ragged, dtype)
     assert all(torch.equal(a, b) for a, b in zip(got, run()))
 
 
+#         B, Tq,  Tk,  H, Hk, D, causal, ragged
+WIDE = [(3, 300, 300, 6, 2, 128, True, True), (2, 65, 700, 2, 2, 72, False, True), (1, 1100, 1100, 2, 1, 120, True, False),
+        (2, 40, 64, 4, 1, 96, True, True), (9, 130, 20, 8, 8, 128, False, True), (1, 33, 129, 3, 3, 104, True, True)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,causal,ragged", WIDE)
+def test_attention_of_wide_heads(B, Tq, Tk, H, Hk, D, causal, ragged, dtype):
+    """Heads of more than 64 features, whose gradients are formed by pairs of waves: one pair a block, two and four, the walk
+    over queries cut and not, tiles that end inside the sequences."""
+    q, do = normal((B, Tq, H, D), 1, dtype), normal((B, Tq, H, D), 2, dtype)
+    k, v = normal((B, Tk, Hk, D), 3, dtype), normal((B, Tk, Hk, D), 4, dtype)
+    lens = None
+    if ragged:
+        lens = torch.randint(0, Tk + 1, (B,), generator=torch.Generator().manual_seed(6))
+        lens[0] = Tk - 1
+        for b in range(B):
+            k[b, lens[b]:] = math.nan
+            v[b, lens[b]:] = math.inf
+    on = None if lens is None else lens.to(DEV)
+    got = run_attention(q, k, v, do, on, causal)
+    want, bound = ref.attention(q, k, v, lens, causal, do=do)
+    for n, a, b, t in zip(("o", "dq", "dk", "dv"), got, want, bound):
+        ref.check(a, b, t, n)
+    assert all(torch.equal(a, b) for a, b in zip(got, run_attention(q, k, v, do, on, causal)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,T,H,Hk,D", [(2, 200, 2, 2, 128), (1, 700, 4, 1, 48), (600, 140, 2, 2, 32)])
+def test_single_gradients_are_those_of_all(B, T, H, Hk, D, dtype):
+    """Every subset of the three gradients has the bits it has when all are asked for."""
+    q, do = normal((B, T, H, D), 1, dtype).to(DEV), normal((B, T, H, D), 2, dtype).to(DEV)
+    k, v = normal((B, T, Hk, D), 3, dtype).to(DEV), normal((B, T, Hk, D), 4, dtype).to(DEV)
+
+    def run(want):
+        leaves = [t.clone().requires_grad_(w) for t, w in zip((q, k, v), want)]
+        attention(*leaves, causal=True).backward(do)
+        return [t.grad for t in leaves]
+
+    every = run((True, True, True))
+    for n in range(1, 7):
+        want = [bool(n & 1), bool(n & 2), bool(n & 4)]
+        for g, e, w in zip(run(want), every, want):
+            assert torch.equal(g, e) if w else g is None
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_reads_nothing_behind_a_length(dtype):
     q, k, v, do = (normal((2, 50, 2, 32), i, dtype) for i in range(4))
@@ -385,11 +431,12 @@ def test_norm_projection_rotary_attention_together():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("N,causal,D", [(3, True, 16), (600, False, 16), (3, False, 24)])
-def test_fused_projection_equals_its_parts(N, causal, D, dtype):
+@pytest.mark.parametrize("N,T,causal,D", [(3, 45, True, 16), (600, 45, False, 16), (3, 45, False, 24), (520, 150, True, 32),
+                                          (2, 300, True, 80)])
+def test_fused_projection_equals_its_parts(N, T, causal, D, dtype):
     """RotarySelfAttentionFn runs the very kernels that rotate and attention run on the parts: the same bits."""
     from speech_amd.functional import RotarySelfAttentionFn
-    T, H = 45, 2
+    H = 2
     turns = rotary_turns(D)[0].to(DEV)
     qkv, do = normal((N, T, 3 * H, D), 1, dtype).to(DEV), normal((N, T, H, D), 2, dtype).to(DEV)
     lens = torch.randint(0, T + 1, (N,), generator=torch.Generator().manual_seed(1)).to(DEV)
