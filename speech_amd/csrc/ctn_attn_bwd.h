@@ -177,8 +177,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 // The same for fp32 heads of 65 to 128 features, whose queries, output gradients (three planes of each) and sums would leave room
 // for one wave a SIMD: 32 queries belong to a pair of waves, one forms the probabilities, the other dP^T - delta.  They
 // exchange the two through LDS in fp32, and each adds the products of one half of the features to its dQ.  16 sequences of 1024
-// causal steps, 8 heads on 2 of 128 features: 312 us, one wave for both 417 us.  (bf16 keys and values are a third as large, and
-// one wave has room for both at two waves a SIMD.)
+// causal steps, 8 heads on 2 of 128 features: 312 us, one wave for both 417 us.  (bf16 queries and gradients are a third as large, and one
+// wave has room for both at two waves a SIMD; so have fp32 heads of 64 features: 270 us, in pairs 336 us, 16 sequences of 1000
+// steps of 8 heads.)
 template <typename T, int DT, int NW>
 __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1))) void attn_dq_pair_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 128, KS = DT / 16, ND = DT / 64, KT = walk_tile<T, DT>();
@@ -510,7 +511,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 // tile: behind the scores, and behind the products that read the tile.  Two waves a SIMD, 32 matrix instructions a wave and
 // tile of 64 queries (bf16): 423 us for one wave with both gradients, 345 us for pairs (bf16, two sequences of 4096 causal
 // steps, 16 heads on 4 of 128 features; 833 TFLOP/s); fp32, 16 sequences of 1024 causal steps, 8 heads on 2: 470 us, 360 us.
-// Giving either wave of a pair the higher priority changes nothing.
+// Heads of 64 features gain nothing in fp32 (354 and 345 us, 16 sequences of 1000 steps of 8 heads) and lose in bf16, where one wave
+// has room for all (103 and 134 us, 8 sequences of 2048 causal steps of 8 heads).  Giving either wave of a pair the higher
+// priority changes nothing.
 template <typename T, int DT, int NW>
 __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 2 : 1))) void attn_dkv_pair_kernel(const bwd_params f) {
     constexpr int NP = Planes<T>::N, NT = NW * 128, KS = DT / 16, ND = DT / 32, QT = walk_tile<T, DT>();
