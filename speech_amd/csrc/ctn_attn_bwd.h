@@ -633,6 +633,9 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
             for (int g = 0; g < 4; ++g)
                 ctn_st4(probs + 1024 * r + 256 * g, f32x4{s[r][4 * g], s[r][4 * g + 1], s[r][4 * g + 2], s[r][4 * g + 3]});
         }
+        // into the buffer that was last read in front of the barrier at the end of the last tile; dK's waves have the time here,
+        // while dV's form exponentials
+        if (i + 1 < i1) stage((i - i0 + 1) & 1);
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < QT / 32; ++r) {
@@ -665,7 +668,6 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(NW == 
                 }
             }
         }
-        if (i + 1 < i1) stage((i - i0 + 1) & 1);
         if (++ct == nq) ct = 0;
         __syncthreads();
     }
