@@ -659,24 +659,24 @@ class RotarySelfAttentionFn(torch.autograd.Function):
     its parts."""
 
     @staticmethod
-    def forward(ctx, qkv, turns, magnitude, lengths, causal):
+    def forward(ctx, qkv, turns, interleaved, magnitude, lengths, causal):
         H = qkv.shape[2] // 3
-        qk, v = ops.rotary(qkv[:, :, :2 * H], turns, magnitude=magnitude), qkv[:, :, 2 * H:]
+        qk, v = ops.rotary(qkv[:, :, :2 * H], turns, None, 0, interleaved, False, magnitude), qkv[:, :, 2 * H:]
         o, lse, low = ops.attn_fwd(qk[:, :, :H], qk[:, :, H:], v, lengths, causal, want_lse=ctx.needs_input_grad[0])
         ctx.save_for_backward(qk, qkv, turns, o, lse, low, lengths)
-        ctx.meta = (magnitude, causal)
+        ctx.meta = (interleaved, magnitude, causal)
         return o
 
     @_differentiated_once
     def backward(ctx, do):
         qk, qkv, turns, o, lse, low, lengths = ctx.saved_tensors
-        magnitude, causal = ctx.meta
+        interleaved, magnitude, causal = ctx.meta
         H = qkv.shape[2] // 3
         dqkv, dqk = torch.empty_like(qkv, memory_format=torch.contiguous_format), torch.empty_like(qk)
         ops.attn_bwd(do, qk[:, :, :H], qk[:, :, H:], qkv[:, :, 2 * H:], o, lse, low, lengths, causal,
                      out=(dqk[:, :, :H], dqk[:, :, H:], dqkv[:, :, 2 * H:]))
-        ops.rotary(dqk, turns, inverse=True, magnitude=magnitude, out=dqkv[:, :, :2 * H])
-        return dqkv, None, None, None, None
+        ops.rotary(dqk, turns, None, 0, interleaved, True, magnitude, dqkv[:, :, :2 * H])
+        return dqkv, None, None, None, None, None
 
 
 # ------------------------------------------------------------------------------------------------ axis shuffles of the dual-path blocks

@@ -50,7 +50,8 @@ class DPRNNTasNet(nn.Module):
         self.sep_norm = sep_norm
         self.mask_nonlinear = mask_nonlinear
         self.rnn_type = rnn_type
-        self.sep_num_heads = kwargs.pop('sep_num_heads', None) or 4        # of rnn_type='attention'
+        num_heads = kwargs.pop('sep_num_heads', None)                      # of rnn_type='attention'
+        self.sep_num_heads = 4 if num_heads is None else num_heads
         self.n_sources = n_sources
         self.eps = eps
 

@@ -111,7 +111,7 @@ class SelfAttention(nn.Module):
 
     def __init__(self, num_features, hidden_channels, num_heads=4, causal=False):
         super().__init__()
-        if hidden_channels % num_heads or (hidden_channels // num_heads) % 8 or hidden_channels // num_heads > 128:
+        if num_heads < 1 or hidden_channels % num_heads or (hidden_channels // num_heads) % 8 or hidden_channels // num_heads > 128:
             raise ValueError("hidden_channels is expected to be num_heads times a multiple of 8 up to 128, but given {} and "
                              "{} heads".format(hidden_channels, num_heads))
         self.num_heads, self.head_dim = num_heads, hidden_channels // num_heads
@@ -123,5 +123,6 @@ class SelfAttention(nn.Module):
         N, T, _ = input.size()
         H, D = self.num_heads, self.head_dim
         qkv = LinearFn.apply(input, self.in_proj.weight, self.in_proj.bias).view(N, T, 3 * H, D)
-        out = RotarySelfAttentionFn.apply(qkv, self.rotary.turns, self.rotary.magnitude, lengths, self.causal)
+        rotary = self.rotary
+        out = RotarySelfAttentionFn.apply(qkv, rotary.turns, rotary.interleaved, rotary.magnitude, lengths, self.causal)
         return out.view(N, T, H * D)

@@ -193,6 +193,17 @@ def test_dual_path_attention_model_config_and_keys(tmp_path):
         DPRNNTasNet(**dict(SMALL, rnn_type='gru'))
 
 
+@pytest.mark.parametrize("hidden,heads", [(32, 0), (32, -1), (32, 3), (24, 2), (288, 2)])
+def test_self_attention_refuses_head_counts(hidden, heads):
+    from dprnn_cases import SMALL
+    from speech_amd.models.dprnn_tasnet import DPRNNTasNet
+    from speech_amd.modules.attention import SelfAttention
+    with pytest.raises(ValueError, match="num_heads times a multiple of 8"):
+        SelfAttention(16, hidden, num_heads=heads)
+    with pytest.raises(ValueError, match="num_heads times a multiple of 8"):
+        DPRNNTasNet(**dict(SMALL, sep_hidden_channels=hidden, rnn_type='attention', sep_num_heads=heads))
+
+
 def test_attention_workspace_of_every_size_the_wrapper_asks_for():
     for code in (_lib.TYPE_F32, _lib.TYPE_BF16):
         assert ops._attn_ws(2, 3, 3, 2, 1, 16, code, False, True) >= 2 * 2 * 3

@@ -7,6 +7,7 @@ import torch
 
 import attention_cases as ref
 from speech_amd._lib import CtnError
+from speech_amd.functional import LinearFn
 from speech_amd.modules.attention import RotaryPositions, SelfAttention, attention, rotary_turns, rotate
 from speech_amd.modules.norm import FrameLayerNorm, frame_layer_norm
 
@@ -441,13 +442,27 @@ def test_fused_projection_equals_its_parts(N, T, causal, D, dtype):
     qkv, do = normal((N, T, 3 * H, D), 1, dtype).to(DEV), normal((N, T, H, D), 2, dtype).to(DEV)
     lens = torch.randint(0, T + 1, (N,), generator=torch.Generator().manual_seed(1)).to(DEV)
     a = qkv.clone().requires_grad_(True)
-    ya = RotarySelfAttentionFn.apply(a, turns, 1.5, lens, causal)
+    ya = RotarySelfAttentionFn.apply(a, turns, N == 3, 1.5, lens, causal)
     ya.backward(do)
     b = qkv.clone().requires_grad_(True)
-    qk = rotate(b[:, :, :2 * H], turns, magnitude=1.5)
+    qk = rotate(b[:, :, :2 * H], turns, interleaved=N == 3, magnitude=1.5)
     yb = attention(qk[:, :, :H], qk[:, :, H:], b[:, :, 2 * H:], lens, causal)
     yb.backward(do)
     assert torch.equal(ya, yb) and torch.equal(a.grad, b.grad)
+
+
+def test_self_attention_takes_its_rotary_module_as_it_is():
+    """Another layout, part of a head and a scaling, put into the module: the output is that of its parts."""
+    torch.manual_seed(1)
+    m = SelfAttention(24, 64, num_heads=2, causal=True).to(DEV)
+    m.rotary = RotaryPositions(32, rotary_dim=16, interleaved=True, scaling=('ramp', 4.0, 512, 1, 32)).to(DEV)
+    x = normal((2, 37, 24), 3).to(DEV)
+    with torch.no_grad():
+        qkv = LinearFn.apply(x, m.in_proj.weight, m.in_proj.bias).view(2, 37, 6, 32)
+        qk = m.rotary(qkv[:, :, :4])
+        want = attention(qk[:, :, :2], qk[:, :, 2:], qkv[:, :, 4:], causal=True).view(2, 37, 64)
+        assert torch.equal(m(x), want)
+    assert torch.equal(m(x), want)
 
 
 def test_second_derivatives_are_refused():
