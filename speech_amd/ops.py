@@ -377,6 +377,13 @@ def _type(t, what):
 
 
 def _same_place(what, first, *rest):
+    device = first.device
+    if first.is_cuda:
+        for t in rest:
+            if t is not None and t.device != device:
+                break
+        else:
+            return
     _require_cuda(first, *rest)
     for t in rest:
         if t is not None and t.device != first.device:
@@ -528,14 +535,15 @@ def check_attention(q, k, v, lengths):
     if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[3] != ks[3]:
         raise _lib.CtnError("attention: q (B, Tq, H, D), k and v (B, Tk, Hk, D), got {}, {}, {}".format(
             tuple(qs), tuple(ks), tuple(v.shape)))
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise _lib.CtnError("attention: q, k and v of one type, got {}, {}, {}".format(q.dtype, k.dtype, v.dtype))
-    H, Hk, D = qs[2], ks[2], qs[3]
+    B, _, H, D = qs
+    Hk = ks[2]
     if Hk < 1 or H < 1 or H % Hk:
         raise _lib.CtnError("attention: {} query heads for {} key heads (a multiple)".format(H, Hk))
     if D % 8 or not 8 <= D <= ATTENTION_MAX_HEAD:
         raise _lib.CtnError("attention: {} features per head (multiples of 8 up to {})".format(D, ATTENTION_MAX_HEAD))
-    if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (qs[0],)):
+    if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != (B,)):
         raise _lib.CtnError("attention: whole lengths of shape ({},), got {} {}".format(
             qs[0], lengths.dtype, tuple(lengths.shape)))
     return code
