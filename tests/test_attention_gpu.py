@@ -535,6 +535,63 @@ def test_captured_steps_replay_like_eager_ones():
                 assert torch.equal(a, b)
 
 
+def test_captured_module_with_lengths_replays_like_eager():
+    """SelfAttention and its input's gradient in a graph; inputs and lengths change between the replays."""
+    torch.manual_seed(2)
+    m = SelfAttention(24, 64, num_heads=2).to(DEV)
+    x = normal((3, 50, 24), 1).to(DEV).requires_grad_(True)
+    lens = torch.tensor([50, 7, 0], device=DEV)
+
+    def step(x, lens):
+        o = m(x, lens)
+        return (o.detach(),) + torch.autograd.grad(o, (x,), torch.ones_like(o))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, lens)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(x, lens)
+    for n in range(3):
+        with torch.no_grad():
+            x.copy_(normal((3, 50, 24), 10 + n))
+            lens.copy_(torch.tensor([n, 50 - n, 33]))
+        g.replay()
+        eager = step(x.detach().clone().requires_grad_(True), lens.clone())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_two_threads_on_two_streams():
+    """Calls from two threads at once, each on a stream of its own: the same bits as alone."""
+    import threading
+    cases = [(normal((2, 150, 4, 32), 1), normal((2, 150, 4, 32), 2)), (normal((3, 90, 2, 128), 3, BF16), normal((3, 90, 2, 128), 4, BF16))]
+    base = [run_attention(q, q, q, do, None, True) for q, do in cases]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(8):
+                    q, do = cases[i]
+                    got[i].append(run_attention(q, q, q, do, None, True))
+                    frame_layer_norm(q.to(DEV))
+            stream.synchronize()
+        except Exception as e:                               # an error in a thread would otherwise pass unseen
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    for i in range(2):
+        assert len(got[i]) == 8 and all(torch.equal(a, b) for r in got[i] for a, b in zip(r, base[i]))
+
+
 def test_calls_on_a_side_stream():
     side = torch.cuda.Stream()
     q, k, v, do = (normal((2, 300, 4, 32), i) for i in range(4))
