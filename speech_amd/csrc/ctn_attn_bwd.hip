@@ -18,8 +18,8 @@ namespace {
 using namespace attn;
 
 // ------------------------------------------------------------------------------------------------ one block per key head
-// Many short fp32 sequences with heads of up to 32 features (the dual-path blocks: thousands of (sequence, head) pairs of a
-// few hundred steps): one block of four waves owns a (batch element, key head) and forms all three gradients in five
+// Many fp32 sequences, or short ones, with heads of up to 32 features (the dual-path blocks: thousands of (sequence, head) pairs
+// of a few hundred steps): one block of four waves owns a (batch element, key head) and forms all three gradients in five
 // products instead of the seven of the two launches above.  The walk is the dK / dV kernel's -- 128 keys at a time, 32 per
 // wave, over the query tiles of every head of the group -- and dQ comes out of the same score gradients: ds has the keys as
 // columns, dQ^T = K^T ds^T wants the queries there, and the matrix instruction itself turns it over, ds^T = ds^T I with ds
@@ -299,9 +299,14 @@ int dkv_pieces(const ctn_attn_args& a, const int nt) {
     return n < 1 ? 1 : n > 16 ? 16 : (int)n;
 }
 
-// One block per key head: where there are four blocks a CU at least.
+// One block per key head: where there are enough of them -- 384, one and a half a CU (256 steps each: 77 us against 84, of 256 heads
+// 58 against 57, of 128 heads 50 against 38; 512 heads of 512 steps: 306 against 351) -- or where the block's walk of 128 keys by
+// 32 queries at a time is short, and one launch with one pair of latencies beats two of them (8 heads of 64 steps: 10 us against 14, of 128: 15
+// against 21; six stages 20 against 24, eight 25 against 25 to 27, sixteen 46 against 32).
 bool whole_fits(const ctn_attn_args& a) {
-    return a.type == CTN_TYPE_F32 && a.D <= 32 && (int64_t)a.batch * a.Hk >= 1024 && a.Tq > 0 && a.Tk > 0;
+    if (a.type != CTN_TYPE_F32 || a.D > 32 || a.Tq == 0 || a.Tk == 0) return false;
+    const int64_t stages = (int64_t)ctn_cdiv(a.Tk, 128) * ctn_cdiv(a.Tq, 32) * (a.H / a.Hk);
+    return (int64_t)a.batch * a.Hk >= 384 || stages <= 6;
 }
 
 int64_t round16(const int64_t n) { return (n + 15) / 16 * 16; }

@@ -249,6 +249,33 @@ def test_attention_of_many_sequences(B, Tq, Tk, H, Hk, D, causal, ragged, dtype)
     assert all(torch.equal(a, b) for a, b in zip(got, run()))
 
 
+#          B, Tq,  Tk,  H, Hk, D, causal, ragged
+SHORT = [(2, 96, 128, 4, 2, 32, True, True), (1, 97, 128, 4, 2, 32, True, False), (3, 192, 100, 2, 2, 24, False, True),
+         (3, 193, 100, 2, 2, 24, False, True), (2, 64, 250, 2, 2, 32, True, True), (1, 1, 700, 1, 1, 8, False, True),
+         (96, 150, 150, 4, 4, 32, True, True), (95, 150, 150, 4, 4, 32, False, False)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,causal,ragged", SHORT)
+def test_attention_of_short_sequences(B, Tq, Tk, H, Hk, D, causal, ragged, dtype):
+    """Both sides of the rules that give a key head's gradients to one block: six stages of 128 keys by 32 queries and seven, 384
+    key heads and fewer."""
+    q, do = normal((B, Tq, H, D), 1, dtype), normal((B, Tq, H, D), 2, dtype)
+    k, v = normal((B, Tk, Hk, D), 3, dtype), normal((B, Tk, Hk, D), 4, dtype)
+    lens = None
+    if ragged:
+        lens = torch.randint(0, Tk + 1, (B,), generator=torch.Generator().manual_seed(7))
+        lens[0] = Tk - 1
+        for b in range(B):
+            k[b, lens[b]:] = math.nan
+            v[b, lens[b]:] = math.inf
+    on = None if lens is None else lens.to(DEV)
+    got = run_attention(q, k, v, do, on, causal)
+    want, bound = ref.attention(q, k, v, lens, causal, do=do)
+    for n, a, b, t in zip(("o", "dq", "dk", "dv"), got, want, bound):
+        ref.check(a, b, t, n)
+
+
 #         B, Tq,  Tk,  H, Hk, D, causal, ragged
 WIDE = [(3, 300, 300, 6, 2, 128, True, True), (2, 65, 700, 2, 2, 72, False, True), (1, 1100, 1100, 2, 1, 120, True, False),
         (2, 40, 64, 4, 1, 96, True, True), (9, 130, 20, 8, 8, 128, False, True), (1, 33, 129, 3, 3, 104, True, True)]
